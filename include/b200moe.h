@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define B200MOE_ABI_VERSION 4
+#define B200MOE_ABI_VERSION 5
 
 /* error codes */
 #define B200MOE_OK 0
@@ -42,10 +42,33 @@ extern "C" {
 #define B200MOE_WEIGHTS_BF16 0
 #define B200MOE_WEIGHTS_W4G128 1 /* packed int4 (q+8), 8 per int32, BF16 scale per 128 along K */
 
+/* element types of operators that take more than BF16 */
+#define B200MOE_BF16 0
+#define B200MOE_FP16 1
+#define B200MOE_FP32 2
+
 /* schedules (shape-only choice, the analogue of moe_full_policy.py:132-152) */
 #define B200MOE_SCHEDULE_AUTO 0
 #define B200MOE_SCHEDULE_GENERIC 1 /* CUDA-core tiles, any H/I */
 #define B200MOE_SCHEDULE_TCGEN05 2 /* TMA + tcgen05/TMEM tiles, needs H%8==0 and I%8==0 */
+
+/* Router configuration. The default router (use_router = 1, and the only one the reference's capture script has,
+ * scripts/capture_qwen3_moe_layer0.py:583-587) is softmax, no groups, renormalised, scale 1. */
+#define B200MOE_SCORE_SOFTMAX 0
+#define B200MOE_SCORE_SIGMOID 1
+#define B200MOE_GROUP_MAX 0  /* a group is worth its largest selection score */
+#define B200MOE_GROUP_TOP2 1 /* ... the sum of its two largest */
+
+typedef struct {
+  int32_t score;        /* B200MOE_SCORE_* over the E logits of a token */
+  int32_t groups;       /* groups of E / groups consecutive experts; 1 = none; at most 32, divides E */
+  int32_t kept_groups;  /* groups a token may choose from; topk <= kept_groups * E / groups */
+  int32_t group_score;  /* B200MOE_GROUP_* */
+  int32_t renormalize;  /* 1: the K weights of a token are divided by their sum */
+  int32_t bf16_weights; /* 1: weights rounded through BF16 */
+  float scale;          /* factor on the weights, > 0 */
+  int32_t reserved;
+} B200MoeRouterConfig;
 
 typedef struct B200MoePlan B200MoePlan;
 
@@ -62,7 +85,8 @@ typedef struct {
   int32_t down_format;    /* B200MOE_WEIGHTS_* */
   int32_t schedule;       /* B200MOE_SCHEDULE_* */
   int32_t token_tile;     /* rows of one expert handled by one tile; 0 = choose from T*K/E */
-  int32_t use_router;     /* 1: ids / routing_weights are written by the router each forward */
+  int32_t use_router;     /* 1: ids / routing_weights are written by the router each forward; 2: by the router that
+                             `router` describes, with the optional bias B200MoeBuffers.router_bias */
   int32_t route_only;     /* 1: no expert weights: forward = router + dispatch; combine reads down_output
                              filled by the caller (the token-owning side of expert parallelism);
                              2: the same, and dispatch does not copy rows (grouped_input may be NULL) */
@@ -92,6 +116,7 @@ typedef struct {
                              (an expert-parallel layer and its single-GPU twin) pin the same value.
                              B200MoeWorkspace.down_tiles reports what the plan resolved. */
   int32_t reserved[1];
+  B200MoeRouterConfig router; /* read when use_router is 2 */
 } B200MoeShape;
 
 /* Bytes of every workspace buffer the caller must allocate (256-byte aligned
@@ -156,6 +181,7 @@ typedef struct {
   const void* ep_row_dest;
   const void* ep_return_bases;
   void* source_rows;           /* [R] int32 workspace, required when the plan gathers (B200MoeWorkspace.gathers) */
+  const void* router_bias;     /* optional [E] float32, added to the scores for the choice of experts (use_router = 2) */
 } B200MoeBuffers;
 
 /* ABI version of the loaded library. */
@@ -194,6 +220,27 @@ int b200moe_dispatch(B200MoePlan* plan, void* cuda_stream);
 int b200moe_gate_up(B200MoePlan* plan, void* cuda_stream);
 int b200moe_down(B200MoePlan* plan, void* cuda_stream);
 int b200moe_combine(B200MoePlan* plan, void* cuda_stream);
+
+/* Routing on logits that the caller has already (no counterpart in the reference, whose operator takes ids and
+ * weights). ids = the K experts of the largest selection score in descending order, ties to the lower index; an
+ * expert whose logit or bias is NaN or -inf is masked: never chosen while another is left, weight 0. The choice is
+ * that of exact arithmetic on the logits; weights are FP32. Every row is written; nothing else is. No workspace:
+ * calls may overlap on the GPU as long as their outputs differ. */
+typedef struct {
+  int32_t tokens;          /* T >= 0 */
+  int32_t experts;         /* 1 <= E <= 256 */
+  int32_t topk;            /* 1 <= K <= 32 */
+  int32_t dtype;           /* of the logits: B200MOE_BF16 / FP16 / FP32 */
+  int32_t ids_are_int64;
+  int32_t reserved;
+  int64_t pitch;           /* elements from one row of logits to the next, >= E */
+  B200MoeRouterConfig config;
+  const void* logits;      /* [T,E] */
+  const void* bias;        /* [E] float32 or NULL */
+  void* ids;               /* [T,K] int32 / int64 */
+  void* weights;           /* [T,K] float32 */
+} B200MoeRouteArgs;
+int b200moe_route(const B200MoeRouteArgs* args, void* cuda_stream);
 
 /* Arguments of b200moe_dispatch_static(): the tensors of the dispatch stage as
  * plain device pointers. Inputs: x [T,H] bf16, ids [T,K] int32/int64,

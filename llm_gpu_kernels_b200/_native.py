@@ -10,7 +10,7 @@ import threading
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libb200moe.so"
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 STATUS_BAD_ID = 1
 STATUS_BAD_WEIGHT = 2
@@ -20,6 +20,8 @@ STATUS_EP_OVERFLOW = 8
 WEIGHTS_BF16 = 0
 WEIGHTS_W4G128 = 1
 
+BF16, FP16, FP32 = 0, 1, 2   # element types of operators that take more than BF16
+
 SCHEDULE_AUTO = 0
 SCHEDULE_GENERIC = 1
 SCHEDULE_TCGEN05 = 2
@@ -28,15 +30,23 @@ SCHEDULE_NAMES = {SCHEDULE_GENERIC: "generic", SCHEDULE_TCGEN05: "tcgen05"}
 ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_STATE = -1, -2, -3, -4
 
 
+class RouterConfig(ctypes.Structure):
+    """``B200MoeRouterConfig``."""
+    _fields_ = [(name, ctypes.c_int32) for name in (
+        "score", "groups", "kept_groups", "group_score", "renormalize", "bf16_weights")] + [
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
 class Shape(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in (
         "tokens", "experts", "topk", "hidden", "intermediate", "ids_are_int64", "gate_up_format",
         "down_format", "schedule", "token_tile", "use_router", "route_only", "external_dispatch", "router_bf16_weights",
-        "unchained", "fused_gather", "down_tiles")] + [("reserved", ctypes.c_int32 * 1)]
+        "unchained", "fused_gather", "down_tiles")] + [("reserved", ctypes.c_int32 * 1), ("router", RouterConfig)]
 
 
 WORKSPACE_BUFFERS = ("output", "counts", "offsets", "cursors", "tasks", "mapping", "ranks",
                      "grouped_input", "activated", "down_output", "status", "scratch")
+
 
 
 class Workspace(ctypes.Structure):
@@ -51,7 +61,15 @@ INPUT_BUFFERS = ("x", "router_weight", "gate_up", "gate_up_scales", "down", "dow
 
 class Buffers(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in INPUT_BUFFERS + WORKSPACE_BUFFERS + (
-        "valid_routes", "residual", "ep_row_dest", "ep_return_bases", "source_rows")]
+        "valid_routes", "residual", "ep_row_dest", "ep_return_bases", "source_rows", "router_bias")]
+
+
+class RouteArgs(ctypes.Structure):
+    """``B200MoeRouteArgs``: routing on given logits."""
+    _fields_ = [(name, ctypes.c_int32) for name in (
+        "tokens", "experts", "topk", "dtype", "ids_are_int64", "reserved")] + [
+        ("pitch", ctypes.c_int64), ("config", RouterConfig)] + [
+        (name, ctypes.c_void_p) for name in ("logits", "bias", "ids", "weights")]
 
 
 class DispatchArgs(ctypes.Structure):
@@ -92,6 +110,7 @@ EXPORTS = {
     "b200moe_gate_up": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "b200moe_down": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "b200moe_combine": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "b200moe_route": (ctypes.c_int, [ctypes.POINTER(RouteArgs), ctypes.c_void_p]),
     "b200moe_dispatch_static": (ctypes.c_int, [ctypes.POINTER(DispatchArgs), ctypes.c_void_p]),
     "b200moe_plan_chain": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p),
                                           ctypes.POINTER(ctypes.c_int32)]),
@@ -144,3 +163,33 @@ def check(code: int):
     if code == ERR_INVALID:
         raise ValueError(message)
     raise RuntimeError(f"b200moe error {code}: {message}")
+
+
+def launch(call, args, device):
+    """``call(args, stream)`` on the current stream of device ``device``; ``args`` is a struct or a plan handle."""
+    import torch
+    arg = ctypes.byref(args) if isinstance(args, ctypes.Structure) else args
+    if torch.cuda.current_device() == device:
+        code = call(arg, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            code = call(arg, torch.cuda.current_stream().cuda_stream)
+    if code:
+        check(code)
+
+
+def _span(t):
+    """First byte and one past the last byte that tensor ``t`` covers."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def check_disjoint(written, read):
+    """A tensor that a kernel writes may not share memory with another one it writes or reads."""
+    written = [t for t in written if t is not None and t.numel()]
+    others = [t for t in read if t is not None and t.numel()]
+    for i, w in enumerate(written):
+        for t in written[:i] + others:
+            a, b = _span(w), _span(t)
+            if a[0] < b[1] and b[0] < a[1]:
+                raise ValueError("an output shares memory with another output or with an input")

@@ -15,7 +15,7 @@ the tensors passed per call for the tracer's benefit and the addresses fixed in 
 from __future__ import annotations
 
 import weakref
-from typing import List
+from typing import List, Optional
 
 import torch
 
@@ -72,4 +72,27 @@ def forward(plan: int, x: torch.Tensor, weights: List[torch.Tensor], ids: torch.
 
 @forward.register_fake
 def _(plan, x, weights, ids, routing_weights, output, workspace):
+    return None
+
+
+@torch.library.custom_op("b200moe::route", mutates_args=("ids", "routing_weights"), device_types="cuda")
+def route(logits: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor, routing_weights: torch.Tensor,
+          score: int, groups: int, kept_groups: int, group_score: int, renormalize: bool, scale: float) -> None:
+    """Routing of given logits (``b200moe_route``) for tracers; ``PreparedRouting.run()`` calls it while compiling."""
+    if logits.shape[0] == 0:
+        return
+    types = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16, torch.float32: _native.FP32}
+    rows = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+    args = _native.RouteArgs(
+        tokens=rows.shape[0], experts=rows.shape[1], topk=ids.shape[1], dtype=types[rows.dtype],
+        ids_are_int64=int(ids.dtype == torch.int64), pitch=rows.stride(0) if rows.shape[0] > 1 else rows.shape[1],
+        config=_native.RouterConfig(score=score, groups=groups, kept_groups=kept_groups, group_score=group_score,
+                                    renormalize=int(renormalize), scale=scale),
+        logits=rows.data_ptr(), bias=bias.data_ptr() if bias is not None else None, ids=ids.data_ptr(),
+        weights=routing_weights.data_ptr())
+    _native.launch(_native.load().b200moe_route, args, rows.device.index)
+
+
+@route.register_fake
+def _(logits, bias, ids, routing_weights, score, groups, kept_groups, group_score, renormalize, scale):
     return None

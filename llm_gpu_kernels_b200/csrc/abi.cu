@@ -155,6 +155,11 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
     set_error("router needs topk <= experts");
     return B200MOE_ERR_INVALID;
   }
+  if (s.use_router < 0 || s.use_router > 2) {
+    set_error("use_router must be 0, 1 (default router) or 2 (the configured one)");
+    return B200MOE_ERR_INVALID;
+  }
+  if (s.use_router == 2 && !route_config_ok(s.router, s.experts, s.topk)) return B200MOE_ERR_INVALID;
   if (s.use_router && router_smem_bytes(s.hidden, s.experts) > 227 * 1024) {
     set_error("router: hidden=%d does not fit the shared-memory staging", s.hidden);
     return B200MOE_ERR_UNSUPPORTED;
@@ -357,6 +362,10 @@ int b200moe_plan_bind(B200MoePlan* p, const B200MoeBuffers* b) {
     }
     if (s.use_router && !b->router_weight) {
       set_error("use_router is set but router_weight is null");
+      return B200MOE_ERR_INVALID;
+    }
+    if (b->router_bias && (s.use_router != 2 || reinterpret_cast<uintptr_t>(b->router_bias) % 4)) {
+      set_error("router_bias belongs to a configured router (use_router = 2) and must be 4-byte aligned");
       return B200MOE_ERR_INVALID;
     }
     // the output and the workspace must not alias the inputs (cuda_gate_up.cu:150-158)

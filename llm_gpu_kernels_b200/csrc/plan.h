@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 #include "../../include/b200moe.h"
+#include "route_row.cuh"
 
 struct B200MoePlan {
   B200MoeShape shape{};
@@ -71,6 +72,15 @@ cudaError_t launch_gate_up_w4r(const B200MoePlan& p, cudaStream_t s, bool chaine
 cudaError_t launch_down_w4r(const B200MoePlan& p, cudaStream_t s, bool chained);
 bool w4r_serves(const B200MoePlan& p);
 cudaError_t launch_combine(const B200MoePlan& p, cudaStream_t s);
+
+// Router configurations: host-side check (sets the error message) and the form the kernels take.
+bool route_config_ok(const B200MoeRouterConfig& c, int experts, int topk);
+route::Config route_config(const B200MoeRouterConfig& c, int experts, int topk);
+inline route::Config route_config(const B200MoePlan& p) {
+  route::Config cfg = route_config(p.shape.router, p.shape.experts, p.shape.topk);
+  cfg.bf16_weights |= p.shape.router_bf16_weights != 0;
+  return cfg;
+}
 
 size_t router_smem_bytes(int hidden, int experts);
 cudaError_t router_opt_in_smem();

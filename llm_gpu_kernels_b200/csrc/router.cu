@@ -6,6 +6,7 @@
 // is the new first stage in front of its fixed-route contract (moe.py:227-230).
 #include <cuda_bf16.h>
 #include "plan.h"
+#include "route_row.cuh"
 
 namespace b200moe {
 namespace {
@@ -19,10 +20,11 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-template <typename IdT>
+template <typename IdT, bool kGeneral>
 __global__ void __launch_bounds__(kRouterThreads)
 router_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ wr,
-                   IdT* __restrict__ ids, float* __restrict__ rw, int T, int E, int H, int K, int bf16_weights) {
+                   IdT* __restrict__ ids, float* __restrict__ rw, int T, int E, int H, int K, int bf16_weights,
+                   const __grid_constant__ route::Config cfg, const float* __restrict__ bias) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   float* xs = reinterpret_cast<float*>(smem_raw);               // [kRouterTokens][H]
   float* logits = xs + static_cast<size_t>(kRouterTokens) * H;   // [kRouterTokens][E]
@@ -81,6 +83,14 @@ router_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __r
   if (warp >= nt) return;
   // one warp per token: softmax, then K rounds of arg-max
   float* l = logits + warp * E;
+  if constexpr (kGeneral) {   // a configured router: route_row.cuh, eight consecutive experts per lane
+    float row[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) row[j] = lane * 8 + j < E ? l[lane * 8 + j] : -INFINITY;
+    const size_t o = static_cast<size_t>(t0 + warp) * K;
+    route::route_row<8, 32, IdT>(cfg, row, bias, lane, 0xffffffffu, ids + o, rw + o);
+    return;
+  }
   float m = -INFINITY;
   for (int e = lane; e < E; e += 32) m = fmaxf(m, l[e]);
 #pragma unroll
@@ -134,12 +144,19 @@ cudaError_t launch_router(const B200MoePlan& p, cudaStream_t s) {
   auto* x = static_cast<const __nv_bfloat16*>(p.buf.x);
   auto* wr = static_cast<const __nv_bfloat16*>(p.buf.router_weight);
   auto* rw = static_cast<float*>(p.buf.routing_weights);
-  if (sh.ids_are_int64) {
-    router_topk_kernel<long long><<<grid, kRouterThreads, smem, s>>>(
-        x, wr, static_cast<long long*>(p.buf.ids), rw, sh.tokens, sh.experts, sh.hidden, sh.topk, sh.router_bf16_weights);
+  auto launch = [&](auto kernel, auto* ids) {
+    kernel<<<grid, kRouterThreads, smem, s>>>(x, wr, ids, rw, sh.tokens, sh.experts, sh.hidden, sh.topk,
+                                              sh.router_bf16_weights, route_config(p),
+                                              static_cast<const float*>(p.buf.router_bias));
+  };
+  auto* ids64 = static_cast<long long*>(p.buf.ids);
+  auto* ids32 = static_cast<int*>(p.buf.ids);
+  if (sh.use_router == 2) {
+    if (sh.ids_are_int64) launch(router_topk_kernel<long long, true>, ids64);
+    else launch(router_topk_kernel<int, true>, ids32);
   } else {
-    router_topk_kernel<int><<<grid, kRouterThreads, smem, s>>>(
-        x, wr, static_cast<int*>(p.buf.ids), rw, sh.tokens, sh.experts, sh.hidden, sh.topk, sh.router_bf16_weights);
+    if (sh.ids_are_int64) launch(router_topk_kernel<long long, false>, ids64);
+    else launch(router_topk_kernel<int, false>, ids32);
   }
   return cudaPeekAtLastError();
 }
@@ -152,9 +169,15 @@ size_t router_smem_bytes(int hidden, int experts) {
 // second plan with a smaller hidden size cannot lower it under the first plan's launches.
 cudaError_t router_opt_in_smem() {
   constexpr int kLimit = 227 * 1024;
-  cudaError_t e = cudaFuncSetAttribute(router_topk_kernel<int>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLimit);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(router_topk_kernel<long long>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLimit);
+  const void* kernels[] = {
+      reinterpret_cast<const void*>(router_topk_kernel<int, false>), reinterpret_cast<const void*>(router_topk_kernel<int, true>),
+      reinterpret_cast<const void*>(router_topk_kernel<long long, false>),
+      reinterpret_cast<const void*>(router_topk_kernel<long long, true>)};
+  for (const void* kernel : kernels) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLimit);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace b200moe

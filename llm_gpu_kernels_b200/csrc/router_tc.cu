@@ -18,6 +18,7 @@
 #include "plan.h"
 #include "sm100_ptx.cuh"
 #include "pdl.cuh"
+#include "route_row.cuh"
 
 namespace b200moe {
 namespace {
@@ -43,11 +44,14 @@ static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block too large");
 
 // kPerLane: experts per lane in the routing epilogue (ceil(E / 32) rounded up to 1, 2, 4 or 8): the top-k rounds
 // walk exactly the keys a lane holds.
-template <typename IdT, int kPerLane>
+// kGeneral: a configured router (score function, bias, groups, ...): the row goes through route_row.cuh, for which a
+// lane holds kPerLane consecutive experts. The default router keeps the code below.
+template <typename IdT, int kPerLane, bool kGeneral>
 __global__ void __launch_bounds__(kThreads, 1)
 router_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_wr,
                  IdT* __restrict__ ids, float* __restrict__ rw, int* __restrict__ status, int T, int E, int H,
-                 int K, int e_pad, int num_stages, int ksplit, int bf16_weights) {
+                 int K, int e_pad, int num_stages, int ksplit, int bf16_weights,
+                 const __grid_constant__ route::Config cfg, const float* __restrict__ bias) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Ctrl* c = reinterpret_cast<Ctrl*>(smem_raw);
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -159,7 +163,27 @@ router_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     for (int rr = warp - 2; rr < rows_per_cta; rr += kRowWarps) {
       const int r = static_cast<int>(cta_rank) * rows_per_cta + rr;
       if (r >= rows_live) break;
-      {
+      if constexpr (kGeneral) {
+        float l[kPerLane];
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j) {
+          const int e = lane * kPerLane + j;
+          l[j] = -INFINITY;
+          if (e < E) {
+            l[j] = 0.0f;
+            for (int sidx = 0; sidx < ksplit; ++sidx) {  // fixed order: slice 0, 1, ...
+              uint32_t remote;
+              asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                           : "=r"(remote) : "r"(logits_addr + static_cast<uint32_t>((r * ld + e) * 4)), "r"(sidx));
+              float part;
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote) : "memory");
+              l[j] += part;
+            }
+          }
+        }
+        const size_t o = static_cast<size_t>(t0 + r) * K;
+        route::route_row<kPerLane, 32, IdT>(cfg, l, bias, lane, 0xffffffffu, ids + o, rw + o);
+      } else {
         // key(x): unsigned, monotonic in x; 0 is below every finite logit and marks "absent / taken"
         uint32_t key[kPerLane];
         uint32_t kmax_local = 0;
@@ -270,12 +294,22 @@ int configure_router_tc(B200MoePlan& p) {
   p.router_smem = kCtrlBytes + 1024 + stages * stage;
   p.router_ksplit = ksplit;
   const void* kernels[] = {
-      reinterpret_cast<const void*>(router_tc_kernel<int, 1>), reinterpret_cast<const void*>(router_tc_kernel<int, 2>),
-      reinterpret_cast<const void*>(router_tc_kernel<int, 4>), reinterpret_cast<const void*>(router_tc_kernel<int, 8>),
-      reinterpret_cast<const void*>(router_tc_kernel<long long, 1>),
-      reinterpret_cast<const void*>(router_tc_kernel<long long, 2>),
-      reinterpret_cast<const void*>(router_tc_kernel<long long, 4>),
-      reinterpret_cast<const void*>(router_tc_kernel<long long, 8>)};
+      reinterpret_cast<const void*>(router_tc_kernel<int, 1, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 2, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 4, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 8, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 1, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 2, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 4, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 8, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 1, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 2, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 4, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 8, false>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 1, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 2, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 4, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 8, true>)};
   for (const void* kernel : kernels) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (e != cudaSuccess) {
@@ -309,12 +343,19 @@ cudaError_t launch_router_typed(const B200MoePlan& p, cudaStream_t s, IdT* ids) 
   auto* rw = static_cast<float*>(p.buf.routing_weights);
   auto launch = [&](auto kernel) {
     return cudaLaunchKernelEx(&cfg, kernel, p.tm_x, p.tm_router_w, ids, rw, status, sh.tokens, sh.experts, sh.hidden,
-                              sh.topk, e_pad, p.router_stages, p.router_ksplit, sh.router_bf16_weights);
+                              sh.topk, e_pad, p.router_stages, p.router_ksplit, sh.router_bf16_weights, route_config(p),
+                              static_cast<const float*>(p.buf.router_bias));
   };
-  if (e_pad <= 32) return launch(router_tc_kernel<IdT, 1>);
-  if (e_pad <= 64) return launch(router_tc_kernel<IdT, 2>);
-  if (e_pad <= 128) return launch(router_tc_kernel<IdT, 4>);
-  return launch(router_tc_kernel<IdT, 8>);
+  if (sh.use_router == 2) {
+    if (sh.experts <= 32) return launch(router_tc_kernel<IdT, 1, true>);
+    if (sh.experts <= 64) return launch(router_tc_kernel<IdT, 2, true>);
+    if (sh.experts <= 128) return launch(router_tc_kernel<IdT, 4, true>);
+    return launch(router_tc_kernel<IdT, 8, true>);
+  }
+  if (e_pad <= 32) return launch(router_tc_kernel<IdT, 1, false>);
+  if (e_pad <= 64) return launch(router_tc_kernel<IdT, 2, false>);
+  if (e_pad <= 128) return launch(router_tc_kernel<IdT, 4, false>);
+  return launch(router_tc_kernel<IdT, 8, false>);
 }
 
 

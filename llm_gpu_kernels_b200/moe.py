@@ -8,10 +8,11 @@ with no allocation, no host read and no synchronisation, so it can be captured
 in a CUDA graph). The kernels behind it are the sm_100a library reached
 through the C ABI of ``include/b200moe.h``; nothing here computes on the host.
 
-Two additions to the reference interface, both keyword-only:
+Additions to the reference interface, all keyword-only:
 ``router_weight`` ([E,H] BF16) puts the top-k softmax router in front of the
 fixed-route path - ``ids`` and ``routing_weights`` then are outputs rewritten by
-every ``run()``; ``schedule`` / ``token_tile`` pin the shape-only kernel choice.
+every ``run()``; ``router`` (a ``RouterConfig``) and ``router_bias`` ([E] FP32) make it
+another router; ``schedule`` / ``token_tile`` pin the shape-only kernel choice.
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ import torch
 
 from . import _native, _ops
 from .gemm import GemmConfig
+from .moe_router import RouterConfig, check_bias
 
 STAGE_NAMES = ("router", "dispatch", "gate_up_swiglu", "down", "combine")
 _GATHER = {False: 1, True: 0, "never": 2}   # keep_grouped_input -> B200MoeShape.fused_gather
@@ -81,6 +83,8 @@ class PreparedMoE:
     ranks: torch.Tensor = None
     scratch: torch.Tensor = None
     router_weight: torch.Tensor = None
+    router: RouterConfig = None          # None: the default router (when there is a router_weight)
+    router_bias: torch.Tensor = None
     gate_up_scales: torch.Tensor = None  # set when gate_up holds packed W4G128 words
     down_scales: torch.Tensor = None     # set when down holds packed W4G128 words
     packed: object = None                # the PackedGateUp the plan was prepared from (reference W4Workspace.packed)
@@ -148,7 +152,8 @@ class PreparedMoE:
             return self.output
         if self._op_args is None:
             weights = [t for t in (self.gate_up, self.down, self.router_weight, self.gate_up_scales,
-                                   self.down_scales, self.valid_routes, self.residual) if t is not None]
+                                   self.down_scales, self.valid_routes, self.residual, self.router_bias)
+                       if t is not None]
             workspace = [self.counts, self.offsets, self.cursors, self.tasks, self.mapping, self.ranks,
                          self.grouped_input, self.activated, self.down_output, self.status, self.scratch]
             if self.source_rows is not None:
@@ -228,7 +233,7 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
              token_tile=0, config=None, warm=True, gate_up_scales=None, down_scales=None,
              route_only_experts=None, valid_routes=None, copy_rows=True, workspace=None,
              router_bf16_weights=False, residual=None, unchained=False, keep_grouped_input=False, down_pair=None,
-             down_tiles=None):
+             down_tiles=None, router=None, router_bias=None):
     """Validate, allocate the workspace, bind the native plan, run one forward.
 
     With ``gate_up_scales`` / ``down_scales`` the matching weight argument is the packed
@@ -245,6 +250,15 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
     if valid_routes is not None and (valid_routes.dtype != torch.int32 or valid_routes.numel() != 1
                                      or valid_routes.device != x.device):
         raise ValueError("valid_routes must be one int32 on the same device")
+    if router is not None and not isinstance(router, RouterConfig):
+        raise TypeError("router must be RouterConfig")
+    if (router is not None or router_bias is not None) and router_weight is None:
+        raise ValueError("router / router_bias configure the router of router_weight, which is missing")
+    if router is None and router_bias is not None:
+        router = RouterConfig()
+    if router is not None:
+        router.check(e, ids.shape[1])
+        check_bias(router_bias, e, x.device)
     if schedule not in _SCHEDULES:
         raise ValueError(f"unknown schedule {schedule!r}; expected one of auto/generic/tcgen05")
     if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape
@@ -258,7 +272,8 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
                           gate_up_format=_native.WEIGHTS_BF16 if gate_up_scales is None else _native.WEIGHTS_W4G128,
                           down_format=_native.WEIGHTS_BF16 if down_scales is None else _native.WEIGHTS_W4G128,
                           schedule=_SCHEDULES[schedule], token_tile=int(token_tile),
-                          use_router=int(router_weight is not None),
+                          use_router=0 if router_weight is None else 1 if router is None else 2,
+                          router=router.native() if router is not None else _native.RouterConfig(),
                           route_only=0 if route_only_experts is None else (1 if copy_rows else 2),
                           router_bf16_weights=int(bool(router_bf16_weights)), unchained=int(bool(unchained)),
                           fused_gather=_GATHER[keep_grouped_input],
@@ -281,7 +296,7 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             bf16((0 if route_only_experts is not None else r, intermediate)), bf16((r, h)),
             int32((1,)), config,
             ranks=int32((r,)), scratch=int32((max(1, sizes.scratch // 4),)), router_weight=router_weight,
-            schedule=_native.SCHEDULE_NAMES[sizes.schedule], token_tile=sizes.token_tile,
+            router=router, router_bias=router_bias, schedule=_native.SCHEDULE_NAMES[sizes.schedule], token_tile=sizes.token_tile,
             kernel_launches=sizes.launches, gate_up_scales=gate_up_scales, down_scales=down_scales,
             valid_routes=valid_routes, residual=residual, gathers=bool(sizes.gathers), down_pair=sizes.down_tiles == 1,
             down_tiles=sizes.down_tiles,
@@ -304,6 +319,7 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             x=ptr(x), router_weight=ptr(router_weight), gate_up=ptr(gate_up), gate_up_scales=ptr(gate_up_scales),
             down=ptr(down), down_scales=ptr(down_scales), ids=ptr(ids), routing_weights=ptr(routing_weights),
             valid_routes=ptr(valid_routes), residual=ptr(residual), source_rows=ptr(plan.source_rows),
+            router_bias=ptr(router_bias),
             **{name: ptr(tensor) for name, tensor in expected.items()})
         with torch.cuda.device(device):
             _native.check(lib.b200moe_plan_bind(handle, ctypes.byref(buffers)))
@@ -324,9 +340,12 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
 
 
 def prepare_moe(x, gate_up, down, ids, routing_weights, *, router_weight=None, schedule=None, token_tile=0,
-                router_bf16_weights=False, residual=None, keep_grouped_input=False, down_pair=None, down_tiles=None):
+                router_bf16_weights=False, residual=None, keep_grouped_input=False, down_pair=None, down_tiles=None,
+                router=None, router_bias=None):
     """Drop-in for reference ``prepare_moe`` (moe.py:220-245). ``router_bf16_weights`` makes the router round
     its weights through BF16 like the captured model does (scripts/capture_qwen3_moe_layer0.py:587-588).
+    ``router`` / ``router_bias`` make the router of ``router_weight`` another one than softmax, top-k, renormalise:
+    sigmoid scores, a balance bias, expert groups, a scale (``moe_router.RouterConfig``).
     ``residual`` ([T,H] bf16, read every forward) is added to the layer result inside the combine kernel:
     ``output = bf16(residual + bf16(layer))``, the model's residual add without a round trip through HBM.
     ``keep_grouped_input=True`` makes every forward fill the ``grouped_input`` workspace tensor as the reference's
@@ -337,7 +356,8 @@ def prepare_moe(x, gate_up, down, ids, routing_weights, *, router_weight=None, s
     ``PreparedMoE.down_tiles`` reports): plans that must agree to the bit pin the same one."""
     return _prepare(x, gate_up, down, ids, routing_weights, router_weight=router_weight, schedule=schedule,
                     token_tile=token_tile, router_bf16_weights=router_bf16_weights, residual=residual,
-                    keep_grouped_input=keep_grouped_input, down_pair=down_pair, down_tiles=down_tiles)
+                    keep_grouped_input=keep_grouped_input, down_pair=down_pair, down_tiles=down_tiles, router=router,
+                    router_bias=router_bias)
 
 
 def _prepare_expert_side(gate_up, down, grouped_input, *, token_tile, gate_up_scales=None, down_scales=None,

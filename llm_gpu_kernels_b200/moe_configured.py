@@ -12,7 +12,7 @@ from .moe_ranked import _ranked
 
 
 def prepare_configured_moe(x, gate_up, down, ids, routing_weights, config, *, router_weight=None,
-                           schedule=None):
+                           schedule=None, router=None, router_bias=None):
     if not isinstance(config, GemmConfig):
         raise TypeError("config must be GemmConfig")
     hidden, intermediate = x.shape[1] if x.ndim == 2 else 0, down.shape[2] if down.ndim == 3 else 0
@@ -24,5 +24,5 @@ def prepare_configured_moe(x, gate_up, down, ids, routing_weights, config, *, ro
             raise ValueError("block_m above 256 exceeds the tcgen05 MMA N range")
         token_tile = config.block_m
     base = _prepare(x, gate_up, down, ids, routing_weights, router_weight=router_weight, schedule=schedule,
-                    token_tile=token_tile, config=config)
+                    token_tile=token_tile, config=config, router=router, router_bias=router_bias)
     return _ranked(base)

@@ -15,13 +15,14 @@ VARIANTS = {"sync": 0, "async": 1, "async_skip": 2}
 
 
 def prepare_cuda_moe(x, gate_up, down, ids, routing_weights, *, variant="sync", down_config=None,
-                     router_weight=None):
+                     router_weight=None, router=None, router_bias=None):
     if variant not in VARIANTS:
         raise ValueError("unsupported CUDA variant")
     if down_config is None:
         return prepare_ranked_moe_launcher(x, gate_up, down, ids, routing_weights, router_weight=router_weight,
-                                           schedule="tcgen05")
+                                           schedule="tcgen05", router=router, router_bias=router_bias)
     if not isinstance(down_config, GemmConfig):
         raise TypeError("down_config must be GemmConfig")
     return prepare_configured_moe(x, gate_up, down, ids, routing_weights, down_config,
-                                  router_weight=router_weight, schedule="tcgen05")
+                                  router_weight=router_weight, schedule="tcgen05", router=router,
+                                  router_bias=router_bias)

@@ -63,12 +63,12 @@ class CudaBackend:
     fixed-route plan (top-1, capacity rows) over the local experts."""
 
     def __init__(self, x, gate_up_local, down_local, ids, routing_weights, *, experts, router_weight, capacity,
-                 global_routes, gate_up_scales=None, down_scales=None):
+                 global_routes, gate_up_scales=None, down_scales=None, router=None, router_bias=None):
         device = x.device
         hidden = x.shape[1]
         local_experts = gate_up_local.shape[0]
         self.token_plan = _prepare(x, None, None, ids, routing_weights, router_weight=router_weight,
-                                   route_only_experts=experts)
+                                   route_only_experts=experts, router=router, router_bias=router_bias)
         self.recv_x = torch.zeros((capacity, hidden), dtype=torch.bfloat16, device=device)
         self.recv_ids = torch.zeros((capacity, 1), dtype=torch.int32, device=device)
         self.recv_rw = torch.ones((capacity, 1), dtype=torch.float32, device=device)
@@ -79,7 +79,8 @@ class CudaBackend:
         tile = token_tile_for(global_routes, experts, 1) if tensor_tiles else 0
         self.expert_plan = _prepare(self.recv_x, gate_up_local, down_local, self.recv_ids, self.recv_rw,
                                     token_tile=tile, valid_routes=self.valid,
-                                    gate_up_scales=gate_up_scales, down_scales=down_scales)
+                                    gate_up_scales=gate_up_scales, down_scales=down_scales, router=router,
+                                 router_bias=router_bias)
         self.local_experts = local_experts
 
     # token-owning side
@@ -178,12 +179,13 @@ class ExpertParallelMoE:
 
 
 def prepare_ep_moe(x, gate_up_local, down_local, ids, routing_weights, *, experts, router_weight=None, group=None,
-                   capacity=None, gate_up_scales=None, down_scales=None):
+                   capacity=None, gate_up_scales=None, down_scales=None, router=None, router_bias=None):
     """Prepare the expert-parallel layer on this rank.
 
     ``x`` [T_local,H] are this rank's tokens; ``gate_up_local`` / ``down_local`` hold only the
     experts of :func:`expert_range`; ``ids`` / ``routing_weights`` [T_local,K] are inputs (global expert
-    ids) or, with ``router_weight`` [E,H], outputs. ``capacity`` = rows this rank can receive
+    ids) or, with ``router_weight`` [E,H] (and ``router`` / ``router_bias``, as ``prepare_moe`` takes them), outputs.
+    ``capacity`` = rows this rank can receive
     (default: every route of every rank, assuming equal token counts).
     """
     world = dist.get_world_size(group)
@@ -195,7 +197,7 @@ def prepare_ep_moe(x, gate_up_local, down_local, ids, routing_weights, *, expert
     capacity = capacity if capacity is not None else max(1, routes * world)
     backend = CudaBackend(x, gate_up_local, down_local, ids, routing_weights, experts=experts,
                           router_weight=router_weight, capacity=capacity, global_routes=max(1, routes * world),
-                          gate_up_scales=gate_up_scales, down_scales=down_scales)
+                          gate_up_scales=gate_up_scales, down_scales=down_scales, router=router, router_bias=router_bias)
     return ExpertParallelMoE(backend, experts=experts, group=group, capacity=capacity)
 
 
@@ -269,7 +271,7 @@ class PeerExpertParallelMoE:
     """Expert-parallel layer whose exchange runs inside the kernels over peer memory."""
 
     def __init__(self, x, gate_up_local, down_local, ids, routing_weights, *, experts, router_weight=None,
-                 group=None, capacity=None, gate_up_scales=None, down_scales=None):
+                 group=None, capacity=None, gate_up_scales=None, down_scales=None, router=None, router_bias=None):
         import ctypes
         from . import _native
         from .moe import _prepare_expert_side
@@ -297,7 +299,7 @@ class PeerExpertParallelMoE:
         ret = ret.view(routes, hidden)
         self.token_plan = _prepare(x, None, None, ids, routing_weights, router_weight=router_weight,
                                    route_only_experts=experts, copy_rows=False, workspace={"down_output": ret},
-                                   warm=False)
+                                   warm=False, router=router, router_bias=router_bias)
         inter = down_local.shape[2] * (8 if down_scales is not None else 1)
         tensor_tiles = hidden % 8 == 0 and inter % 8 == 0 and hidden >= 64 and inter >= 64
         tile = token_tile_for(max(1, routes * self.world), experts, 1) if tensor_tiles else 0
@@ -368,9 +370,11 @@ def ctypes_byref(obj):
 
 
 def prepare_peer_ep_moe(x, gate_up_local, down_local, ids, routing_weights, *, experts, router_weight=None,
-                        group=None, capacity=None, gate_up_scales=None, down_scales=None):
+                        group=None, capacity=None, gate_up_scales=None, down_scales=None, router=None,
+                        router_bias=None):
     """Expert-parallel layer with the exchange fused into the dispatch / return kernels over NVLink
     peer memory. Same arguments as :func:`prepare_ep_moe`. Call ``close()`` before the process group goes away."""
     return PeerExpertParallelMoE(x, gate_up_local, down_local, ids, routing_weights, experts=experts,
                                  router_weight=router_weight, group=group, capacity=capacity,
-                                 gate_up_scales=gate_up_scales, down_scales=down_scales)
+                                 gate_up_scales=gate_up_scales, down_scales=down_scales, router=router,
+                                 router_bias=router_bias)

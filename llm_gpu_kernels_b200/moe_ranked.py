@@ -45,9 +45,10 @@ def _ranked(base: PreparedMoE) -> PreparedRankedMoE:
 
 def prepare_ranked_moe_launcher(x, gate_up, down, ids, routing_weights, *, router_weight=None,
                                 schedule=None, token_tile=0, router_bf16_weights=False, residual=None,
-                                keep_grouped_input=False, down_pair=None, down_tiles=None):
+                                keep_grouped_input=False, down_pair=None, down_tiles=None, router=None,
+                                router_bias=None):
     """Drop-in for reference ``prepare_ranked_moe_launcher`` (moe_ranked.py:99-169)."""
     return _ranked(_prepare(x, gate_up, down, ids, routing_weights, router_weight=router_weight,
                             schedule=schedule, token_tile=token_tile, router_bf16_weights=router_bf16_weights,
                             residual=residual, keep_grouped_input=keep_grouped_input, down_pair=down_pair,
-                            down_tiles=down_tiles))
+                            down_tiles=down_tiles, router=router, router_bias=router_bias))

@@ -27,7 +27,7 @@ def _check_format(packed, what):
 
 
 def prepare_w4_moe(x, packed, down, ids, routing_weights, *, down_config=None, packed_down=None,
-                   router_weight=None, keep_grouped_input=False):
+                   router_weight=None, keep_grouped_input=False, router=None, router_bias=None):
     """Prepare outside timing; no dense weight reconstruction, no counts read-back.
 
     ``down`` is the BF16 ``[E,H,I]`` tensor, or ``None`` when ``packed_down`` is given.
@@ -51,6 +51,6 @@ def prepare_w4_moe(x, packed, down, ids, routing_weights, *, down_config=None, p
         x, packed.words, down if packed_down is None else packed_down.words, ids, routing_weights,
         router_weight=router_weight, schedule="tcgen05", token_tile=token_tile, config=down_config,
         gate_up_scales=packed.scales, down_scales=None if packed_down is None else packed_down.scales,
-        keep_grouped_input=keep_grouped_input)
+        keep_grouped_input=keep_grouped_input, router=router, router_bias=router_bias)
     base.packed = packed
     return _ranked(base)

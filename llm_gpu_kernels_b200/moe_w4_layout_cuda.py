@@ -15,7 +15,7 @@ from .moe_weight_quant import PackedGateUp
 
 
 def prepare_w4_layout_moe(x, repacked, down, ids, routing_weights, *, down_config=None, packed_down=None,
-                          router_weight=None):
+                          router_weight=None, router=None, router_bias=None):
     if not isinstance(repacked, RepackedGateUp):
         raise TypeError("RepackedGateUp required")
     metadata = repacked.metadata
@@ -26,6 +26,7 @@ def prepare_w4_layout_moe(x, repacked, down, ids, routing_weights, *, down_confi
     words, scales = restore_v1_tensors(repacked.words, repacked.scales)
     canonical = PackedGateUp(words, scales, deepcopy(metadata["canonical_v1_metadata"]))
     prepared = prepare_w4_moe(x, canonical, down, ids, routing_weights, down_config=down_config,
-                              packed_down=packed_down, router_weight=router_weight)
+                              packed_down=packed_down, router_weight=router_weight, router=router,
+                              router_bias=router_bias)
     prepared.base.repacked = repacked
     return prepared
