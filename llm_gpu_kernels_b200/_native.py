@@ -166,11 +166,12 @@ def check(code: int):
 
 
 def launch(call, args, device):
-    """``call(args, stream)`` on the current stream of device ``device``; ``args`` is a struct or a plan handle."""
+    """``call(args, stream)`` on the current stream of device ``device``; ``args`` is a struct or a plan handle. Kept
+    short: for one token the kernels behind it take less time than this function."""
     import torch
     arg = ctypes.byref(args) if isinstance(args, ctypes.Structure) else args
-    if torch.cuda.current_device() == device:
-        code = call(arg, torch.cuda.current_stream().cuda_stream)
+    if torch._C._cuda_getDevice() == device:
+        code = call(arg, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
             code = call(arg, torch.cuda.current_stream().cuda_stream)

@@ -1,5 +1,5 @@
 // Routing on given logits: [T, E] in BF16, FP16 or FP32 (rows may be strided) to ids and weights [T, K]. The formula is
-// in route_row.cuh; a row is held in registers by 32, 16, 8 or 4 lanes, up to 8 experts each, and read once.
+// in route_row.cuh; a row is held in registers by 32, 16, 8 or 4 lanes, up to 8 experts each, and read from HBM once.
 // Bound by HBM only for long prompts (32768 x 256 FP32: 33.5 MB in, 2 MB out, floor 5.4 us); at a serving batch one
 // launch is all there is.
 #include <cuda_bf16.h>
@@ -17,83 +17,113 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
-// kVec: a lane's P logits are one aligned piece (E a multiple of P, row pitch and base aligned to P elements).
-template <typename T, typename IdT, int P, int L, bool kVec>
-__global__ void __launch_bounds__(kThreads)
-route_kernel(const T* __restrict__ logits, long long pitch, const float* __restrict__ bias, IdT* __restrict__ ids,
-             float* __restrict__ weights, int tokens, const __grid_constant__ route::Config cfg) {
+// N floats or halves of one lane as FP32: one or two vector loads (N * sizeof(T) of 8, 16 or 32 bytes) or N scalar ones.
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* src, float (&v)[N]) {
+  constexpr int kBytes = N * sizeof(T);
+  union { T t[N]; uint32_t w[(kBytes + 3) / 4]; } raw;
+  if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i) {
+      const uint4 q = *(reinterpret_cast<const uint4*>(src) + i);
+      raw.w[4 * i] = q.x; raw.w[4 * i + 1] = q.y; raw.w[4 * i + 2] = q.z; raw.w[4 * i + 3] = q.w;
+    }
+  } else if constexpr (kBytes == 8) {
+    const uint2 q = *reinterpret_cast<const uint2*>(src);
+    raw.w[0] = q.x; raw.w[1] = q.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw.t[i] = src[i];
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = to_float(raw.t[j]);
+}
+
+// kVec: a lane's P logits, and its P biases, are each one aligned piece.
+template <typename T, int P, int L, bool kVec>
+__global__ void __launch_bounds__(kThreads, 8)   // 64 registers: the rare FP64 pass may spill, the common one does not
+route_kernel(const T* __restrict__ logits, long long pitch, const float* __restrict__ bias, void* __restrict__ ids,
+             int ids_are_int64, float* __restrict__ weights, int tokens, const __grid_constant__ route::Config cfg) {
   pdl_launch_dependents();
   pdl_wait();   // the logits may come from the kernel just before; ids / weights may still be read by it
   const int lane = threadIdx.x & (L - 1);
-  const long long row = static_cast<long long>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
-  if (row >= tokens) return;
-  const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) & ~(L - 1));
-  const T* src = logits + row * pitch + lane * P;
-  float l[P];
+  const long long wanted = static_cast<long long>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
+  const bool live = wanted < tokens;
+  const long long row = live ? wanted : tokens - 1;   // lanes past the end follow the last row and write nothing
+  const T* row_logits = logits + row * pitch;
+  float l[P], b[P];
+  const bool inside = lane * P < cfg.E;
   if (kVec) {
-    union { T v[P]; uint32_t w[(P * sizeof(T) + 3) / 4]; } raw;
-    if (lane * P < cfg.E) {
-      constexpr int kBytes = P * sizeof(T);
-      if constexpr (kBytes % 16 == 0) {
 #pragma unroll
-        for (int i = 0; i < kBytes / 16; ++i) {
-          const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
-          raw.w[4 * i] = q.x; raw.w[4 * i + 1] = q.y; raw.w[4 * i + 2] = q.z; raw.w[4 * i + 3] = q.w;
-        }
-      } else if constexpr (kBytes == 8) {
-        const uint2 q = __ldg(reinterpret_cast<const uint2*>(src));
-        raw.w[0] = q.x; raw.w[1] = q.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < P; ++i) raw.v[i] = src[i];
-      }
-#pragma unroll
-      for (int j = 0; j < P; ++j) l[j] = to_float(raw.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < P; ++j) l[j] = -INFINITY;
+    for (int j = 0; j < P; ++j) {
+      l[j] = -INFINITY;
+      b[j] = 0.0f;
     }
+    if (inside) load_vec(row_logits + lane * P, l);
+    if (inside && bias != nullptr) load_vec(bias + lane * P, b);
   } else {
 #pragma unroll
-    for (int j = 0; j < P; ++j) l[j] = lane * P + j < cfg.E ? to_float(src[j]) : -INFINITY;
+    for (int j = 0; j < P; ++j) l[j] = lane * P + j < cfg.E ? to_float(row_logits[lane * P + j]) : -INFINITY;
+    route::load_bias<P>(cfg, bias, lane, b);
   }
-  route::route_row<P, L, IdT>(cfg, l, bias, lane, mask, ids + row * cfg.K, weights + row * cfg.K);
+  const long long first = row * cfg.K;
+  const route::Out out{ids_are_int64 ? static_cast<void*>(static_cast<long long*>(ids) + first)
+                                     : static_cast<void*>(static_cast<int*>(ids) + first), weights + first, ids_are_int64};
+  route::route_row<P, L>(cfg, l, b, bias, lane, live, [&](int e) { return to_float(row_logits[e]); }, out);
 }
 
-template <typename T, typename IdT, int P, int L>
+template <typename T, int P, int L>
 cudaError_t launch(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStream_t s) {
   const T* logits = static_cast<const T*>(a.logits);
-  const bool vec = cfg.E % P == 0 && a.pitch % P == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
-                   (a.pitch * sizeof(T)) % (P * sizeof(T) < 16 ? P * sizeof(T) : 16) == 0;
+  auto* bias = static_cast<const float*>(a.bias);
+  auto* w = static_cast<float*>(a.weights);
+  constexpr bool kPow2 = (P & (P - 1)) == 0;
+  const size_t piece = P * sizeof(T) < 16 ? P * sizeof(T) : 16;
+  const bool vec = kPow2 && cfg.E % P == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
+                   (a.pitch * sizeof(T)) % piece == 0 && reinterpret_cast<uintptr_t>(bias) % 16 == 0;
   const int rows = kThreads / L;
   const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.tokens) + rows - 1) / rows));
-  auto* ids = static_cast<IdT*>(a.ids);
-  auto* w = static_cast<float*>(a.weights);
-  auto* bias = static_cast<const float*>(a.bias);
-  return vec ? launch_pdl(route_kernel<T, IdT, P, L, true>, grid, dim3(kThreads), 0, s, logits,
-                          static_cast<long long>(a.pitch), bias, ids, w, a.tokens, cfg)
-             : launch_pdl(route_kernel<T, IdT, P, L, false>, grid, dim3(kThreads), 0, s, logits,
-                          static_cast<long long>(a.pitch), bias, ids, w, a.tokens, cfg);
+  const long long pitch = a.pitch;
+  if constexpr (kPow2)
+    if (vec)
+      return launch_pdl(route_kernel<T, P, L, true>, grid, dim3(kThreads), 0, s, logits, pitch, bias, a.ids,
+                        a.ids_are_int64, w, a.tokens, cfg);
+  return launch_pdl(route_kernel<T, P, L, false>, grid, dim3(kThreads), 0, s, logits, pitch, bias, a.ids, a.ids_are_int64,
+                    w, a.tokens, cfg);
 }
 
-// Lanes per row: eight experts per lane where that leaves at least four lanes, so that small expert counts share a
-// warp among several rows. Groups need the whole warp (one lane per group).
-template <typename T, typename IdT>
-cudaError_t launch_shape(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStream_t s) {
-  if (cfg.groups > 1 || cfg.E > 128) {
-    if (cfg.E <= 32) return launch<T, IdT, 1, 32>(a, cfg, s);
-    if (cfg.E <= 64) return launch<T, IdT, 2, 32>(a, cfg, s);
-    if (cfg.E <= 128) return launch<T, IdT, 4, 32>(a, cfg, s);
-    return launch<T, IdT, 8, 32>(a, cfg, s);
+// Lanes and experts per lane. Few lanes per row, so that rows share a warp (the instructions of a round are then paid
+// once for several rows), but at least K: a lane per weight. With groups, the first pair that gives every group a power
+// of two of whole lanes; where there is none the kernel takes its general pass.
+template <typename T, int L>
+cudaError_t launch_lanes(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStream_t s) {
+  const int size = cfg.size;
+  auto fits = [&](int p) {
+    const int lanes = size / p;
+    return p * L >= cfg.E && (cfg.kept == cfg.groups || (size % p == 0 && (lanes & (lanes - 1)) == 0));
+  };
+  if constexpr (L >= 16) {
+    if (cfg.kept < cfg.groups) {
+      if (fits(1)) return launch<T, 1, L>(a, cfg, s);
+      if (fits(3)) return launch<T, 3, L>(a, cfg, s);
+      if (fits(5)) return launch<T, 5, L>(a, cfg, s);
+      if (fits(6)) return launch<T, 6, L>(a, cfg, s);
+      if (fits(7)) return launch<T, 7, L>(a, cfg, s);
+    }
   }
-  if (cfg.E <= 32) return launch<T, IdT, 8, 4>(a, cfg, s);
-  if (cfg.E <= 64) return launch<T, IdT, 8, 8>(a, cfg, s);
-  return launch<T, IdT, 8, 16>(a, cfg, s);
+  if (fits(2)) return launch<T, 2, L>(a, cfg, s);
+  if (fits(4)) return launch<T, 4, L>(a, cfg, s);
+  return launch<T, 8, L>(a, cfg, s);
 }
 
 template <typename T>
 cudaError_t launch_typed(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStream_t s) {
-  return a.ids_are_int64 ? launch_shape<T, long long>(a, cfg, s) : launch_shape<T, int>(a, cfg, s);
+  if (cfg.kept == cfg.groups) {
+    if (cfg.E <= 32 && cfg.K <= 4) return launch_lanes<T, 4>(a, cfg, s);
+    if (cfg.E <= 64 && cfg.K <= 8) return launch_lanes<T, 8>(a, cfg, s);
+  }
+  if (cfg.E <= 128 && cfg.K <= 16) return launch_lanes<T, 16>(a, cfg, s);
+  return launch_lanes<T, 32>(a, cfg, s);
 }
 
 }  // namespace
@@ -131,6 +161,7 @@ route::Config route_config(const B200MoeRouterConfig& c, int experts, int topk) 
   cfg.sigmoid = c.score == B200MOE_SCORE_SIGMOID;
   cfg.groups = c.groups;
   cfg.kept = c.kept_groups;
+  cfg.size = c.groups > 0 ? experts / c.groups : experts;   // 0 groups: a plan without a configured router
   cfg.group_top2 = c.group_score == B200MOE_GROUP_TOP2;
   cfg.renormalize = c.renormalize != 0;
   cfg.bf16_weights = c.bf16_weights != 0;

@@ -13,9 +13,18 @@
 //
 // Precision: the weights are FP32. The CHOICE is that of exact arithmetic: where c comes from exp() in FP32, two
 // values closer than the error bound of that computation could be in the wrong order, so a row in which two
-// neighbours of the order (or the groups at the border) are that close is routed again in FP64. That is one row in
-// about a thousand for random logits and costs nothing measurable; an FP64 pass for every row would take the
-// 32768 x 256 case from HBM-bound to several times its time.
+// neighbours of the order (or the groups at the border) are that close is routed again in FP64 (route_exact): one row
+// in a few hundred for random logits.
+//
+// What bounds the common pass (route_fast) at many rows is the number of instructions per row, so it keeps the experts
+// of a lane as sorted 32-bit keys: the order-preserving bits of c, of which the lowest three are replaced by the place
+// in the lane. Sorting eight is 19 compare-exchanges of two integer min / max; each of the K rounds is one maximum
+// over the lanes, one ballot and a shift of the winner's list. The K weights are computed at the end by K lanes at
+// once, from logits read again, so full-precision exp and division cost one instruction sequence per row.
+// 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups: 80 us with unsorted keys and per-expert weights (1930 warp
+// instructions per row), 47 us like this (910 instructions; 5.4 us would be the HBM floor). Sixteen experts per lane and
+// two rows per warp need as many instructions per row (935: the warp-wide redux of 32 lanes becomes four shuffles) and
+// more registers: 73 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -28,6 +37,7 @@ struct Config {
   int E, K;
   int sigmoid;      // 0: softmax scores
   int groups, kept; // groups = 1: no groups
+  int size;         // experts of a group
   int group_top2;   // 0: a group's value is its largest c
   int renormalize;
   int bf16_weights; // weights rounded through BF16
@@ -35,9 +45,10 @@ struct Config {
 };
 
 constexpr int kMaxGroups = 32;
-// |c_fp32 - c| <= kScoreError * max(1, |c|): expf within 2 ulp, 13 additions of the softmax sum (up to 8 per lane and
-// 5 levels of the tree), one division and the bias addition are below 17 half-ulps = 1.1e-6; rounded up.
-constexpr float kScoreError = 1.5e-6f;
+// |c_fp32 - c| <= kScoreError * (s_max + |c|) as route_fast computes c: __expf within 2^-22 + |l| 2^-23 relative
+// (weighted by the score: |d| exp(d) <= 0.37), up to 13 additions of a softmax sum (8 in a lane, 5 levels of the tree),
+// an approximate division and the bias addition stay below 1.5e-6; the three dropped key bits are 7 ulp, 8.4e-7 of |c|.
+constexpr float kScoreError = 2.5e-6f;
 
 template <typename F> struct Key;
 template <> struct Key<float> {
@@ -61,243 +72,363 @@ template <> struct Key<double> {
   }
 };
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-
+// The L lanes of a row take part in every step together with the other rows of the warp: control flow is the same for
+// the whole warp, and shuffles name all of it (a mask per row costs extra instructions at every shuffle).
+constexpr unsigned kAll = 0xffffffffu;
 template <int L, typename V>
-__device__ __forceinline__ V sub_max(V v, unsigned mask) {
+__device__ __forceinline__ V sub_max(V v) {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(mask, v, o));
+  for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kAll, v, o));
   return v;
 }
 template <>
-__device__ __forceinline__ uint32_t sub_max<32, uint32_t>(uint32_t v, unsigned) {
-  return __reduce_max_sync(0xffffffffu, v);
+__device__ __forceinline__ uint32_t sub_max<32, uint32_t>(uint32_t v) {
+  return __reduce_max_sync(kAll, v);
 }
 template <int L, typename V>
-__device__ __forceinline__ V sub_sum(V v, unsigned mask) {
+__device__ __forceinline__ V sub_sum(V v) {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
 }
+// Lanes of this row for which p holds, as the low L bits.
+template <int L>
+__device__ __forceinline__ unsigned sub_ballot(bool p) {
+  const unsigned all = __ballot_sync(kAll, p);
+  if (L == 32) return all;
+  return (all >> (threadIdx.x & 31 & ~(L - 1))) & ((1u << (L & 31)) - 1u);
+}
 
-template <typename F>
-__device__ __forceinline__ F minus_inf() { return static_cast<F>(-INFINITY); }
+__device__ __forceinline__ int lowest_lane(unsigned lanes) { return __ffs(static_cast<int>(lanes)) - 1; }
 
-// Which of this lane's experts may be chosen after the group step: bit j. `v` holds c (or the logit) of the
-// candidates of `ok`, `s` the scores. Full warp (L = 32). Sets *close when FP32 cannot decide the border.
-template <typename F, int P>
-__device__ __forceinline__ unsigned keep_groups(const Config& cfg, const F (&v)[P], const F (&s)[P], unsigned ok,
-                                                int lane, bool by_score, bool inexact, bool* close) {
-  const int size = cfg.E / cfg.groups;
-  const F none = minus_inf<F>();
-  F mine = none;                          // lane g: value of group g
-  const int lanes = size / P;             // lanes per group where groups end at lane borders
-  if (size % P == 0 && (lanes & (lanes - 1)) == 0) {
-    F a = none, b = none;                 // the two largest of this lane, then of its group
+// ids may be int32 or int64
+struct Out {
+  void* ids;
+  float* weights;
+  int wide;
+  __device__ __forceinline__ void put(const Config& cfg, int slot, int e, float w) const {
+    if (wide) static_cast<long long*>(ids)[slot] = e;
+    else static_cast<int*>(ids)[slot] = e;
+    weights[slot] = cfg.bf16_weights ? __bfloat162float(__float2bfloat16_rn(w)) : w;
+  }
+};
+
+// Score of one logit; top and sum are those of the softmax (sum = 1 leaves it unnormalised). Masked logits are -inf.
+__device__ __forceinline__ double score_of(const Config& cfg, double x, double top, double sum) {
+  if (cfg.sigmoid) return 1.0 / (1.0 + exp(-x));                 // 0 for -inf
+  return x == -INFINITY ? 0.0 : exp(x == top ? 0.0 : x - top) / sum;
+}
+
+// ------------------------------------------------------------------------------------------------ FP64, any row
+// load(e): the logit of expert e; wanted: this row is to be written (the other rows of the warp only take part). Not inlined: the rare pass must not cost the common one registers; it keeps one
+// 64-bit key per expert and computes the rest when needed.
+template <int P, int L, typename Load>
+__device__ __noinline__ void route_exact(const Config& cfg, const float* __restrict__ bias, int lane, bool wanted,
+                                         const Load& load, const Out& out) {
+  using K = Key<double>;
+  using KeyT = K::type;
+  const double none = -INFINITY;
+  auto logit = [&](int e) { return e < cfg.E ? fmaxf(load(e), -INFINITY) : -INFINITY; };   // NaN -> -inf
+  double top = none, sum = 0.0;
+  if (!cfg.sigmoid) {
+#pragma unroll 1
+    for (int j = 0; j < P; ++j) top = max(top, static_cast<double>(logit(lane * P + j)));
+    top = sub_max<L>(top);
+#pragma unroll 1
+    for (int j = 0; j < P; ++j) sum += score_of(cfg, logit(lane * P + j), top, 1.0);
+    sum = sub_sum<L>(sum);
+  }
+  KeyT key[P];   // 0: not a candidate
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const F x = (ok >> j & 1u) ? (by_score ? s[j] : v[j]) : none;
-      b = max(b, min(a, x));
-      a = max(a, x);
+  for (int j = 0; j < P; ++j) {
+    const int e = lane * P + j;
+    const double x = logit(e);
+    key[j] = 0;
+    if (x > none) {
+      const double b = bias != nullptr ? bias[e] : 0.0;
+      if (b > none) key[j] = K::of(bias != nullptr ? score_of(cfg, x, top, sum) + b : x);   // false for NaN
     }
-    for (int o = 1; o < lanes; o <<= 1) {
-      const F oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-      b = max(min(a, oa), max(b, ob));
-      a = max(a, oa);
-    }
-    const F value = cfg.group_top2 && b != none ? a + b : a;
-    mine = __shfl_sync(0xffffffffu, value, (lane * lanes) & 31);
-    if (lane >= cfg.groups) mine = none;
-  } else {
+  }
+  if (cfg.kept < cfg.groups) {
+    const int size = cfg.size;
+    double mine[kMaxGroups / L];          // lane i holds the values of groups i, i + L, ...
     for (int g = 0; g < cfg.groups; ++g) {
-      F a = none, b = none;
+      KeyT a = 0, b = 0;                  // the two largest of the group
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         const int e = lane * P + j;
-        const F x = (ok >> j & 1u) && e >= g * size && e < (g + 1) * size ? (by_score ? s[j] : v[j]) : none;
+        const KeyT x = e >= g * size && e < (g + 1) * size ? key[j] : 0;
         b = max(b, min(a, x));
         a = max(a, x);
       }
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const F oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+      for (int o = 1; o < L; o <<= 1) {
+        const KeyT oa = __shfl_xor_sync(kAll, a, o), ob = __shfl_xor_sync(kAll, b, o);
         b = max(min(a, oa), max(b, ob));
         a = max(a, oa);
       }
-      if (lane == g) mine = cfg.group_top2 && b != none ? a + b : a;
-    }
-  }
-  int before = 0;                         // groups ordered before this lane's
-  for (int g = 0; g < cfg.groups; ++g) {
-    const F other = __shfl_sync(0xffffffffu, mine, g);
-    before += other > mine || (other == mine && g < lane) ? 1 : 0;
-  }
-  const bool in = lane < cfg.groups, kept = in && before < cfg.kept;
-  if (inexact) {
-    F low = kept ? mine : static_cast<F>(INFINITY), high = in && !kept ? mine : none;
+      double value = none;
+      if (a) {
+        value = K::value(a);
+        if (cfg.group_top2) {
+          const bool scores = bias == nullptr;   // c is the score then, the keys are logits
+          if (scores) value = score_of(cfg, value, top, sum);
+          if (b) value += scores ? score_of(cfg, K::value(b), top, sum) : K::value(b);
+        }
+      }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-      high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+      for (int i = 0; i < kMaxGroups / L; ++i)
+        if (g == lane + i * L) mine[i] = value;
     }
-    F size_of = 1;   // the error of a value goes by the c it is made of, not by their sum
+    unsigned kept_groups = 0;
+    for (int g = 0; g < cfg.groups; ++g) {
+      double value = 0;
+#pragma unroll
+      for (int i = 0; i < kMaxGroups / L; ++i)
+        if (g / L == i) value = mine[i];
+      value = __shfl_sync(kAll, value, g & (L - 1), L);
+      int before = 0;                     // groups ordered before g
+#pragma unroll
+      for (int i = 0; i < kMaxGroups / L; ++i) {
+        const int other = lane + i * L;
+        if (other < cfg.groups) before += mine[i] > value || (mine[i] == value && other < g) ? 1 : 0;
+      }
+      before = sub_sum<L>(before);
+      kept_groups |= before < cfg.kept ? 1u << g : 0u;
+    }
 #pragma unroll
     for (int j = 0; j < P; ++j)
-      if (ok >> j & 1u) size_of = max(size_of, abs(v[j]));
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) size_of = max(size_of, __shfl_xor_sync(0xffffffffu, size_of, o));
-    // each value is a sum of up to two c; infinities compare false
-    if (low - high <= static_cast<F>(4 * kScoreError) * size_of) *close = true;
+      if (key[j] && !(kept_groups >> ((lane * P + j) / size) & 1u)) key[j] = 0;
   }
-  const unsigned groups = __ballot_sync(0xffffffffu, kept);
-  unsigned keep = 0;
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const int e = lane * P + j;
-    if (e < cfg.E && (groups >> (e / size) & 1u)) keep |= 1u << j;
-  }
-  return keep;
-}
-
-// One pass in precision F. Returns false when (F = float) two values are too close for it.
-template <typename F, int P, int L, typename IdT>
-__device__ bool route_pass(const Config& cfg, const float (&l)[P], const float* __restrict__ bias, int lane,
-                           unsigned mask, IdT* __restrict__ ids, float* __restrict__ weights) {
-  using K = Key<F>;
-  using KeyT = typename K::type;
-  constexpr bool kFast = sizeof(F) == 4;
-  const F none = minus_inf<F>();
-  unsigned ok = 0;
-  F v[P], s[P];
-  F top = none;
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const int e = lane * P + j;
-    v[j] = static_cast<F>(l[j]);
-    if (e < cfg.E && l[j] > -INFINITY) {   // false for NaN
-      ok |= 1u << j;
-      top = max(top, v[j]);
-    }
-  }
-  const bool by_score = cfg.groups > 1 && cfg.group_top2 && bias == nullptr;   // group values only
-  const bool scores_first = bias != nullptr || by_score;
-  if (!cfg.sigmoid) {
-    top = sub_max<L>(top, mask);
-    F sum = 0;
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      s[j] = (ok >> j & 1u) ? exp_of(v[j] == top ? static_cast<F>(0) : v[j] - top) : static_cast<F>(0);
-      sum += s[j];
-    }
-    if (scores_first || !cfg.renormalize) {   // otherwise the sum cancels
-      sum = sub_sum<L>(sum, mask);
-#pragma unroll
-      for (int j = 0; j < P; ++j) s[j] = (ok >> j & 1u) ? s[j] / sum : static_cast<F>(0);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < P; ++j) s[j] = (ok >> j & 1u) ? 1 / (1 + exp_of(-v[j])) : static_cast<F>(0);
-  }
-  if (bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const int e = lane * P + j;
-      const float b = e < cfg.E ? bias[e] : 0.0f;
-      v[j] = s[j] + static_cast<F>(b);
-      if (!(b > -INFINITY)) ok &= ~(1u << j);
-    }
-  }
-  bool close = false;
-  if (L == 32 && cfg.groups > 1) ok &= keep_groups<F, P>(cfg, v, s, ok, lane, by_score, kFast && scores_first, &close);
-  KeyT key[P];
-  int rank[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    key[j] = (ok >> j & 1u) ? K::of(v[j]) : static_cast<KeyT>(0);   // 0: not a candidate
-    rank[j] = -1;
-  }
-  const bool check = kFast && bias != nullptr;
-  KeyT last = 0;
-  F total = 0;
+  int expert = 0;                         // lane k: the expert of slot k
+  bool filled = false;
+  unsigned chosen = 0;                    // of this lane's experts
   for (int k = 0; k < cfg.K; ++k) {
     KeyT best = key[0];
 #pragma unroll
     for (int j = 1; j < P; ++j) best = max(best, key[j]);
-    const KeyT winner = sub_max<L>(best, mask);
-    if (winner == 0) {                       // nobody left: the lowest indices not chosen, weight 0
-      for (; k < cfg.K; ++k) {
-        int e = 0x7fffffff;
+    const KeyT winner = sub_max<L>(best);
+    const bool empty = winner == 0;       // nobody left: the lowest index not chosen yet, with weight 0
+    int place = 0;                        // of the winner among this lane's experts, if it is here
 #pragma unroll
-        for (int j = P - 1; j >= 0; --j)
-          if (rank[j] < 0 && lane * P + j < cfg.E) e = lane * P + j;
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) e = min(e, __shfl_xor_sync(mask, e, o));
-#pragma unroll
-        for (int j = 0; j < P; ++j)
-          if (lane * P + j == e) { rank[j] = k; s[j] = 0; }
-      }
-      break;
+    for (int j = P - 1; j >= 0; --j)
+      if (empty ? !(chosen >> j & 1u) : key[j] == winner) place = j;
+    const bool holds = empty ? chosen != (1u << P) - 1u && lane * P + place < cfg.E : best == winner;
+    const int owner = lowest_lane(sub_ballot<L>(holds));   // the lowest lane holds the lowest index
+    place = __shfl_sync(kAll, place, owner, L);
+    if (lane == k) {
+      expert = owner * P + place;
+      filled = !empty;
     }
-    if (check && k > 0) {
-      const F a = K::value(last), b = K::value(winner);
-      if (a - b <= static_cast<F>(2 * kScoreError) * max(static_cast<F>(1), abs(a))) close = true;
-    }
-    last = winner;
-    const unsigned holders = __ballot_sync(mask, best == winner) & mask;
-    bool mine = (holders & (0u - holders)) == 1u << (threadIdx.x & 31);   // the lowest lane holds the lowest index
+    if (lane == owner) {
+      chosen |= 1u << place;
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      if (mine && key[j] == winner) {
-        key[j] = 0;
-        rank[j] = k;
-        total += s[j];
-        mine = false;
-      }
+      for (int j = 0; j < P; ++j)
+        if (j == place) key[j] = 0;
     }
   }
-  if (check) {   // the first expert left out
-    KeyT best = key[0];
-#pragma unroll
-    for (int j = 1; j < P; ++j) best = max(best, key[j]);
-    best = sub_max<L>(best, mask);
-    const F a = K::value(last), b = K::value(best);
-    if (best != 0 && a - b <= static_cast<F>(2 * kScoreError) * max(static_cast<F>(1), abs(a))) close = true;
-  }
-  if (close) return false;
+  double w = lane < cfg.K && filled ? score_of(cfg, logit(expert), top, sum) : 0.0;
   if (cfg.renormalize) {
-    total = sub_sum<L>(total, mask);
-    if (kFast && !(total >= static_cast<F>(1e-30))) return false;   // scores this small have lost their ratio in FP32
+    const double total = sub_sum<L>(w);
+    w = total > 0 ? w / total : 0.0;
   }
-  const F factor = static_cast<F>(cfg.scale);
+  if (wanted && lane < cfg.K) out.put(cfg, lane, expert, static_cast<float>(w * static_cast<double>(cfg.scale)));
+}
+
+// ------------------------------------------------------------------------------------------------ FP32
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b) {
+  const uint32_t hi = max(a, b);
+  b = min(a, b);
+  a = hi;
+}
+// Descending, by Batcher's odd-even merge network for 8 of which the exchanges beyond P fall away (a missing element
+// would be smaller than any other and stay at the end).
+template <int P>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[P]) {
+#pragma unroll
+  for (int p = 1; p < 8; p *= 2)
+#pragma unroll
+    for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+      for (int j = d % p; j + d < 8; j += 2 * d)
+#pragma unroll
+        for (int i = 0; i < d; ++i)
+          if (i + j + d < P && (i + j) / (2 * p) == (i + j + d) / (2 * p)) exchange(k[i + j], k[i + j + d]);
+}
+
+constexpr uint32_t kPlaceBits = 7u;          // P <= 8
+constexpr uint32_t kNoneKey = 0x007fffffu;   // Key<float>::of(-INFINITY); every candidate's key is larger
+
+// Returns false when FP32 cannot settle the row; otherwise slot `lane` < K of the row is `expert` with weight `w`.
+// l[j]: logits of experts lane*P + j, b[j]: biases.
+template <int P, int L, typename Load>
+__device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], const float (&b)[P], bool biased, int lane,
+                                           const Load& load, int* expert, float* weight) {
+  using K = Key<float>;
+  const float none = -INFINITY;
+  const bool grouped = cfg.kept < cfg.groups;
+  uint32_t key[P];
+  uint32_t low_bits = 0;
+  float top = none;
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    if (rank[j] >= 0) {
-      F w = s[j];
-      if (cfg.renormalize) w = total > 0 ? w / total : static_cast<F>(0);
-      float r = static_cast<float>(w * factor);
-      if (cfg.bf16_weights) r = __bfloat162float(__float2bfloat16_rn(r));
-      ids[rank[j]] = static_cast<IdT>(lane * P + j);
-      weights[rank[j]] = r;
+    l[j] = fmaxf(l[j], none);   // NaN -> -inf
+    low_bits |= __float_as_uint(l[j]);
+    top = fmaxf(top, l[j]);
+  }
+  float unit = 1.0f, sum = 1.0f, widest = 0.0f;   // unit: the largest score there can be
+  if (!cfg.sigmoid) {
+    const uint32_t t = sub_max<L>(K::of(top));
+    top = K::value(t);
+    if (biased || grouped || !cfg.renormalize) {
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < P; ++j) sum += l[j] > none ? __expf(l[j] == top ? 0.0f : l[j] - top) : 0.0f;
+      sum = sub_sum<L>(sum);
+      unit = __fdividef(1.0f, sum);
     }
   }
-  return true;
+  auto score = [&](float x) {   // approximate; for the choice only
+    return cfg.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x)) : unit * __expf(x == top ? 0.0f : x - top);
+  };
+  if (biased) {
+    if (cfg.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        key[j] = K::of(fmaxf(l[j] > none ? __fdividef(1.0f, 1.0f + __expf(-l[j])) + b[j] : none, none));
+    } else {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        key[j] = K::of(fmaxf(l[j] > none ? unit * __expf(l[j] == top ? 0.0f : l[j] - top) + b[j] : none, none));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) key[j] = K::of(l[j]);
+  }
+  // without a bias c is the logit itself: nothing is lost if its last bits are zero anyway (16-bit logits, even as FP32)
+  const bool exact = !biased && sub_ballot<L>((low_bits & kPlaceBits) != 0) == 0;
+#pragma unroll
+  for (int j = 0; j < P; ++j) key[j] = (key[j] & ~kPlaceBits) | (kPlaceBits - j);
+  sort_keys<P>(key);
+  bool close = false;
+  if (grouped) {
+    const int lanes = cfg.size / P;   // a whole power of two: see route_row
+    float a = K::value(key[0] & ~kPlaceBits), second = P > 1 ? K::value(key[P > 1] & ~kPlaceBits) : none;
+    a = key[0] > kNoneKey ? a : none;
+    second = P > 1 && key[P > 1] > kNoneKey ? second : none;
+    for (int o = 1; o < lanes; o <<= 1) {
+      const float oa = __shfl_xor_sync(kAll, a, o), ob = __shfl_xor_sync(kAll, second, o);
+      second = fmaxf(fminf(a, oa), fmaxf(second, ob));
+      a = fmaxf(a, oa);
+    }
+    const bool by_score = cfg.group_top2 && !biased;
+    float value = a;
+    if (cfg.group_top2 && a != none) {
+      if (by_score) value = score(a);
+      if (second != none) value += by_score ? score(second) : second;
+    }
+    const int leader = lane & ~(lanes - 1);   // of this lane's group
+    uint32_t group_key = lane == leader && lane * P < cfg.E ? K::of(value) : 0u;
+    bool kept = false;
+    uint32_t last = 0;
+    for (int g = 0; g < cfg.kept; ++g) {
+      last = sub_max<L>(group_key);
+      const int winner = lowest_lane(sub_ballot<L>(group_key == last));
+      kept |= leader == winner;
+      if (lane == winner) group_key = 0u;
+    }
+    if (__any_sync(kAll, !exact) || by_score) {   // is the border between the kept groups and the others certain?
+      const uint32_t next = sub_max<L>(group_key);
+      if (biased || by_score) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) widest = fmaxf(widest, fabsf(b[j]));
+        widest = __uint_as_float(sub_max<L>(__float_as_uint(widest)));
+        close = K::value(last) - K::value(next) <= 4.0f * kScoreError * (unit + widest);   // infinities compare false
+      } else {
+        close = !exact && last == next && last != kNoneKey;
+      }
+    }
+    if (!kept) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) key[j] = 0u;
+    }
+  }
+  // K rounds, and one more where the border matters; sub-lane k keeps the winner of round k
+  uint32_t taken = 0, border = 0;
+  int owner_of = 0;
+  const int rounds = __all_sync(kAll, exact) ? cfg.K : cfg.K + 1;
+  for (int k = 0; k < rounds; ++k) {
+    const uint32_t winner = sub_max<L>(key[0] | kPlaceBits);
+    const int owner = lowest_lane(sub_ballot<L>((key[0] | kPlaceBits) == winner));   // lowest index of a tie
+    border = winner;
+    const uint32_t head = __shfl_sync(kAll, key[0], owner, L);
+    if (lane == k) {
+      taken = head;
+      owner_of = owner;
+    }
+    if (lane == owner) {
+#pragma unroll
+      for (int j = 0; j + 1 < P; ++j) key[j] = key[j + 1];
+      key[P - 1] = 0u;
+    }
+  }
+  const uint32_t won = taken | kPlaceBits;
+  const uint32_t below = __shfl_down_sync(kAll, won, 1, L);
+  const uint32_t next = lane == cfg.K - 1 ? border : below;
+  if (!exact && lane < cfg.K && next > (kNoneKey | kPlaceBits)) {
+    if (biased) {
+      const float x = K::value(won & ~kPlaceBits), y = K::value(next & ~kPlaceBits);
+      close |= x - y <= 2.0f * kScoreError * (unit + fabsf(x));
+    } else {
+      close |= won == next;
+    }
+  }
+  const bool empty = lane < cfg.K && won <= (kNoneKey | kPlaceBits);
+  const unsigned unfilled = sub_ballot<L>(empty);
+  const bool nothing = (unfilled & 1u) != 0;   // a row whose mask leaves nothing: the lowest indices with weight 0
+  const unsigned undecided = sub_ballot<L>(close);   // by every lane: not behind a condition that rows differ in
+  bool settled = nothing || (undecided == 0 && unfilled == 0);
+  *expert = nothing ? lane : owner_of * P + static_cast<int>(kPlaceBits - (taken & kPlaceBits));
+  float w = 0.0f;
+  if (lane < cfg.K && settled && !nothing) {
+    const float x = load(*expert);
+    w = cfg.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x == top ? 0.0f : x - top);
+  }
+  if (cfg.renormalize) {
+    const float total = sub_sum<L>(w);
+    settled = settled && (nothing || total >= 1e-30f);   // scores below that have lost their ratio in FP32
+    w = nothing ? 0.0f : w / total;
+  } else if (!cfg.sigmoid) {
+    w = nothing ? 0.0f : w / sum;
+  }
+  *weight = w * cfg.scale;
+  return settled;
 }
 
-// Not inlined: the rare pass must not cost the common one registers.
-template <int P, int L, typename IdT>
-__device__ __noinline__ void route_again(const Config& cfg, const float (&l)[P], const float* __restrict__ bias, int lane,
-                                         unsigned mask, IdT* __restrict__ ids, float* __restrict__ weights) {
-  route_pass<double, P, L, IdT>(cfg, l, bias, lane, mask, ids, weights);
+// Routes the rows of a warp, 32 / L of them: lane (0..L-1 of its row's lanes) holds logits and biases of experts
+// lane*P .. lane*P+P-1 of its row; load(e) gives a logit of it again. The whole warp calls it; rows that are not
+// `live` (their lanes hold any logits, and load() is called for them) are not written. P * L >= E, L >= K. Groups that
+// do not end at lane borders with a power of two of lanes each go through the general pass.
+template <int P, int L, typename Load>
+__device__ __forceinline__ void route_row(const Config& cfg, float (&l)[P], const float (&b)[P],
+                                          const float* __restrict__ bias, int lane, bool live, const Load& load,
+                                          const Out& out) {
+  const int size = cfg.size, lanes = size / P;
+  const bool lane_groups = cfg.kept == cfg.groups || (size % P == 0 && (lanes & (lanes - 1)) == 0);
+  bool settled = false;
+  if (lane_groups) {
+    int expert;
+    float w;
+    settled = route_fast<P, L>(cfg, l, b, bias != nullptr, lane, load, &expert, &w);
+    if (live && settled && lane < cfg.K) out.put(cfg, lane, expert, w);
+  }
+  if (__any_sync(kAll, live && !settled)) route_exact<P, L>(cfg, bias, lane, live && !settled, load, out);
 }
 
-// Routes one row: lane (0..L-1 of the row's lanes, which are the lanes of `mask`) holds the logits of experts
-// lane*P .. lane*P+P-1 in l; ids / weights point at the row's K entries. P * L >= E; groups > 1 needs L = 32.
-template <int P, int L, typename IdT>
-__device__ __forceinline__ void route_row(const Config& cfg, const float (&l)[P], const float* __restrict__ bias, int lane,
-                                          unsigned mask, IdT* __restrict__ ids, float* __restrict__ weights) {
-  if (!route_pass<float, P, L, IdT>(cfg, l, bias, lane, mask, ids, weights))
-    route_again<P, L, IdT>(cfg, l, bias, lane, mask, ids, weights);
+template <int P>
+__device__ __forceinline__ void load_bias(const Config& cfg, const float* __restrict__ bias, int lane, float (&b)[P]) {
+#pragma unroll
+  for (int j = 0; j < P; ++j) b[j] = bias != nullptr && lane * P + j < cfg.E ? bias[lane * P + j] : 0.0f;
 }
 
 }  // namespace route

@@ -84,11 +84,13 @@ router_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __r
   // one warp per token: softmax, then K rounds of arg-max
   float* l = logits + warp * E;
   if constexpr (kGeneral) {   // a configured router: route_row.cuh, eight consecutive experts per lane
-    float row[8];
+    float row[8], b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) row[j] = lane * 8 + j < E ? l[lane * 8 + j] : -INFINITY;
+    route::load_bias<8>(cfg, bias, lane, b);
     const size_t o = static_cast<size_t>(t0 + warp) * K;
-    route::route_row<8, 32, IdT>(cfg, row, bias, lane, 0xffffffffu, ids + o, rw + o);
+    route::route_row<8, 32>(cfg, row, b, bias, lane, true, [&](int e) { return l[e]; },
+                            route::Out{ids + o, rw + o, sizeof(IdT) == 8});
     return;
   }
   float m = -INFINITY;

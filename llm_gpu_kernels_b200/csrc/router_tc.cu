@@ -164,25 +164,25 @@ router_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
       const int r = static_cast<int>(cta_rank) * rows_per_cta + rr;
       if (r >= rows_live) break;
       if constexpr (kGeneral) {
-        float l[kPerLane];
-#pragma unroll
-        for (int j = 0; j < kPerLane; ++j) {
-          const int e = lane * kPerLane + j;
-          l[j] = -INFINITY;
-          if (e < E) {
-            l[j] = 0.0f;
-            for (int sidx = 0; sidx < ksplit; ++sidx) {  // fixed order: slice 0, 1, ...
-              uint32_t remote;
-              asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                           : "=r"(remote) : "r"(logits_addr + static_cast<uint32_t>((r * ld + e) * 4)), "r"(sidx));
-              float part;
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote) : "memory");
-              l[j] += part;
-            }
+        auto logit = [&](int e) {
+          float sum_parts = 0.0f;
+          for (int sidx = 0; sidx < ksplit; ++sidx) {  // fixed order: slice 0, 1, ...
+            uint32_t remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                         : "=r"(remote) : "r"(logits_addr + static_cast<uint32_t>((r * ld + e) * 4)), "r"(sidx));
+            float part;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote) : "memory");
+            sum_parts += part;
           }
-        }
+          return sum_parts;
+        };
+        float l[kPerLane], b[kPerLane];
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j) l[j] = lane * kPerLane + j < E ? logit(lane * kPerLane + j) : -INFINITY;
+        route::load_bias<kPerLane>(cfg, bias, lane, b);
         const size_t o = static_cast<size_t>(t0 + r) * K;
-        route::route_row<kPerLane, 32, IdT>(cfg, l, bias, lane, 0xffffffffu, ids + o, rw + o);
+        route::route_row<kPerLane, 32>(cfg, l, b, bias, lane, true, logit,
+                                       route::Out{ids + o, rw + o, sizeof(IdT) == 8});
       } else {
         // key(x): unsigned, monotonic in x; 0 is below every finite logit and marks "absent / taken"
         uint32_t key[kPerLane];
@@ -300,7 +300,11 @@ int configure_router_tc(B200MoePlan& p) {
       reinterpret_cast<const void*>(router_tc_kernel<int, 8, false>),
       reinterpret_cast<const void*>(router_tc_kernel<int, 1, true>),
       reinterpret_cast<const void*>(router_tc_kernel<int, 2, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 3, true>),
       reinterpret_cast<const void*>(router_tc_kernel<int, 4, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 5, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 6, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<int, 7, true>),
       reinterpret_cast<const void*>(router_tc_kernel<int, 8, true>),
       reinterpret_cast<const void*>(router_tc_kernel<long long, 1, false>),
       reinterpret_cast<const void*>(router_tc_kernel<long long, 2, false>),
@@ -308,7 +312,11 @@ int configure_router_tc(B200MoePlan& p) {
       reinterpret_cast<const void*>(router_tc_kernel<long long, 8, false>),
       reinterpret_cast<const void*>(router_tc_kernel<long long, 1, true>),
       reinterpret_cast<const void*>(router_tc_kernel<long long, 2, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 3, true>),
       reinterpret_cast<const void*>(router_tc_kernel<long long, 4, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 5, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 6, true>),
+      reinterpret_cast<const void*>(router_tc_kernel<long long, 7, true>),
       reinterpret_cast<const void*>(router_tc_kernel<long long, 8, true>)};
   for (const void* kernel : kernels) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
@@ -347,10 +355,16 @@ cudaError_t launch_router_typed(const B200MoePlan& p, cudaStream_t s, IdT* ids) 
                               static_cast<const float*>(p.buf.router_bias));
   };
   if (sh.use_router == 2) {
-    if (sh.experts <= 32) return launch(router_tc_kernel<IdT, 1, true>);
-    if (sh.experts <= 64) return launch(router_tc_kernel<IdT, 2, true>);
-    if (sh.experts <= 128) return launch(router_tc_kernel<IdT, 4, true>);
-    return launch(router_tc_kernel<IdT, 8, true>);
+    switch ((sh.experts + 31) / 32) {   // groups of a power-of-two number of lanes wherever their size allows it
+      case 1: return launch(router_tc_kernel<IdT, 1, true>);
+      case 2: return launch(router_tc_kernel<IdT, 2, true>);
+      case 3: return launch(router_tc_kernel<IdT, 3, true>);
+      case 4: return launch(router_tc_kernel<IdT, 4, true>);
+      case 5: return launch(router_tc_kernel<IdT, 5, true>);
+      case 6: return launch(router_tc_kernel<IdT, 6, true>);
+      case 7: return launch(router_tc_kernel<IdT, 7, true>);
+      default: return launch(router_tc_kernel<IdT, 8, true>);
+    }
   }
   if (e_pad <= 32) return launch(router_tc_kernel<IdT, 1, false>);
   if (e_pad <= 64) return launch(router_tc_kernel<IdT, 2, false>);
