@@ -41,6 +41,9 @@ extern "C" {
 /* weight formats */
 #define B200MOE_WEIGHTS_BF16 0
 #define B200MOE_WEIGHTS_W4G128 1 /* packed int4 (q+8), 8 per int32, BF16 scale per 128 along K */
+#define B200MOE_WEIGHTS_INT8 2   /* int8, one FP32 scale per output channel; the activations are quantised to int8
+                                    with one scale per row. Weight rows have a pitch of K rounded up to 16 bytes.
+                                    Both projections take this format or neither does. */
 
 /* element types of operators that take more than BF16 */
 #define B200MOE_BF16 0
@@ -131,12 +134,16 @@ typedef struct {
   size_t mapping;       /* [R] int32 */
   size_t ranks;         /* [R] int32 */
   size_t grouped_input; /* [R,H] bf16 */
-  size_t activated;     /* [R,I] bf16 */
+  size_t activated;     /* [R,I] bf16; INT8 plans: [R,I] float32, quantised into activated_q */
   size_t down_output;   /* [R,H] bf16 */
   size_t status;        /* [1] int32 */
   size_t scratch;       /* dispatch partial histograms, router flag, tile counter and per-expert completion
                            counters of the chained GEMM kernels */
   size_t source_rows;   /* [R] int32: token whose row each grouped row is (inverse of mapping; 0 unless gathers) */
+  size_t x_q;           /* INT8 plans: [T, H rounded up to 16] int8, x quantised row by row; else 0 */
+  size_t x_scale;       /* INT8 plans: [T] float32 */
+  size_t activated_q;   /* INT8 plans: [R, I rounded up to 16] int8 */
+  size_t activated_scale; /* INT8 plans: [R] float32 */
   int32_t token_tile;   /* resolved tile */
   int32_t schedule;     /* resolved schedule */
   int32_t launches;     /* kernels one forward enqueues */
@@ -150,10 +157,10 @@ typedef struct {
 typedef struct {
   const void* x;               /* [T,H] bf16 */
   const void* router_weight;   /* [E,H] bf16, NULL unless use_router */
-  const void* gate_up;         /* bf16 [E,2I,H]  or packed int32 [E,2I,H/8] */
-  const void* gate_up_scales;  /* bf16 [E,2I,H/128] for W4G128, else NULL */
-  const void* down;            /* bf16 [E,H,I]   or packed int32 [E,H,I/8] */
-  const void* down_scales;     /* bf16 [E,H,I/128] for W4G128, else NULL */
+  const void* gate_up;         /* bf16 [E,2I,H]  or packed int32 [E,2I,H/8]  or int8 [E,2I,H rounded up to 16] */
+  const void* gate_up_scales;  /* bf16 [E,2I,H/128] for W4G128, float32 [E,2I] for INT8, else NULL */
+  const void* down;            /* bf16 [E,H,I]   or packed int32 [E,H,I/8]   or int8 [E,H,I rounded up to 16] */
+  const void* down_scales;     /* bf16 [E,H,I/128] for W4G128, float32 [E,H] for INT8, else NULL */
   void* ids;                   /* [T,K] int32/int64 (input, or router output) */
   void* routing_weights;       /* [T,K] float32 (input, or router output) */
   void* output;
@@ -182,6 +189,10 @@ typedef struct {
   const void* ep_return_bases;
   void* source_rows;           /* [R] int32 workspace, required when the plan gathers (B200MoeWorkspace.gathers) */
   const void* router_bias;     /* optional [E] float32, added to the scores for the choice of experts (use_router = 2) */
+  void* x_q;                   /* workspace of INT8 plans, see B200MoeWorkspace */
+  void* x_scale;
+  void* activated_q;
+  void* activated_scale;
 } B200MoeBuffers;
 
 /* ABI version of the loaded library. */
@@ -241,6 +252,40 @@ typedef struct {
   void* weights;           /* [T,K] float32 */
 } B200MoeRouteArgs;
 int b200moe_route(const B200MoeRouteArgs* args, void* cuda_stream);
+
+/* One dense product in 8-bit integers: q = rint(127 x / max|row|), y = (q . W^T) * row scale * channel scale, integer
+ * sums, rounded once to the type of x. A row with an infinity or a NaN gives NaN. No counterpart in the reference.
+ * Life cycle as a plan's: create (shape), workspace (sizes), bind (addresses), forward (enqueue only), destroy. */
+typedef struct B200MoeLinear B200MoeLinear;
+typedef struct {
+  int32_t tokens; /* T >= 0 */
+  int32_t k;      /* inputs, 1 <= k <= 131072 (the integer sums must fit 32 bits) */
+  int32_t n;      /* outputs, >= 1 */
+  int32_t dtype;  /* of x and y: B200MOE_BF16 / FP16 */
+  int32_t reserved[4];
+} B200MoeLinearShape;
+typedef struct {
+  size_t x_q;     /* [T, k rounded up to 16] int8 */
+  size_t x_scale; /* [T] float32 */
+  size_t status;  /* [1] int32 */
+  int32_t launches;
+  int32_t reserved;
+} B200MoeLinearWorkspace;
+typedef struct {
+  const void* x;            /* [T,k], rows x_pitch elements apart */
+  int64_t x_pitch;
+  const void* weight;       /* [n, k rounded up to 16] int8, 16-byte aligned */
+  const void* weight_scale; /* [n] float32 */
+  void* output;             /* [T,n] contiguous */
+  void* x_q;                /* workspace */
+  void* x_scale;
+  void* status;             /* zeroed by the caller once; B200MOE_STATUS_TIMEOUT is raised in it */
+} B200MoeLinearBuffers;
+int b200moe_linear_create(const B200MoeLinearShape* shape, B200MoeLinear** linear);
+int b200moe_linear_workspace(const B200MoeLinear* linear, B200MoeLinearWorkspace* sizes);
+int b200moe_linear_bind(B200MoeLinear* linear, const B200MoeLinearBuffers* buffers);
+int b200moe_linear_forward(B200MoeLinear* linear, void* cuda_stream);
+void b200moe_linear_destroy(B200MoeLinear* linear);
 
 /* Arguments of b200moe_dispatch_static(): the tensors of the dispatch stage as
  * plain device pointers. Inputs: x [T,H] bf16, ids [T,K] int32/int64,

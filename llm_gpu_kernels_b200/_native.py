@@ -9,6 +9,8 @@ import ctypes
 import threading
 from pathlib import Path
 
+import torch
+
 LIBRARY_PATH = Path(__file__).resolve().parent / "libb200moe.so"
 ABI_VERSION = 5
 
@@ -19,6 +21,7 @@ STATUS_EP_OVERFLOW = 8
 
 WEIGHTS_BF16 = 0
 WEIGHTS_W4G128 = 1
+WEIGHTS_INT8 = 2
 
 BF16, FP16, FP32 = 0, 1, 2   # element types of operators that take more than BF16
 
@@ -47,10 +50,11 @@ class Shape(ctypes.Structure):
 WORKSPACE_BUFFERS = ("output", "counts", "offsets", "cursors", "tasks", "mapping", "ranks",
                      "grouped_input", "activated", "down_output", "status", "scratch")
 
+INT8_BUFFERS = ("x_q", "x_scale", "activated_q", "activated_scale")
 
 
 class Workspace(ctypes.Structure):
-    _fields_ = [(name, ctypes.c_size_t) for name in WORKSPACE_BUFFERS + ("source_rows",)] + [
+    _fields_ = [(name, ctypes.c_size_t) for name in WORKSPACE_BUFFERS + ("source_rows",) + INT8_BUFFERS] + [
         ("token_tile", ctypes.c_int32), ("schedule", ctypes.c_int32), ("launches", ctypes.c_int32),
         ("gathers", ctypes.c_int32), ("down_tiles", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
@@ -61,7 +65,7 @@ INPUT_BUFFERS = ("x", "router_weight", "gate_up", "gate_up_scales", "down", "dow
 
 class Buffers(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in INPUT_BUFFERS + WORKSPACE_BUFFERS + (
-        "valid_routes", "residual", "ep_row_dest", "ep_return_bases", "source_rows", "router_bias")]
+        "valid_routes", "residual", "ep_row_dest", "ep_return_bases", "source_rows", "router_bias") + INT8_BUFFERS]
 
 
 class RouteArgs(ctypes.Structure):
@@ -70,6 +74,21 @@ class RouteArgs(ctypes.Structure):
         "tokens", "experts", "topk", "dtype", "ids_are_int64", "reserved")] + [
         ("pitch", ctypes.c_int64), ("config", RouterConfig)] + [
         (name, ctypes.c_void_p) for name in ("logits", "bias", "ids", "weights")]
+
+
+class LinearShape(ctypes.Structure):
+    """``B200MoeLinearShape``: one dense product in 8-bit integers."""
+    _fields_ = [(name, ctypes.c_int32) for name in ("tokens", "k", "n", "dtype")] + [("reserved", ctypes.c_int32 * 4)]
+
+
+class LinearWorkspace(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_size_t) for name in ("x_q", "x_scale", "status")] + [
+        ("launches", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class LinearBuffers(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("x_pitch", ctypes.c_int64)] + [
+        (name, ctypes.c_void_p) for name in ("weight", "weight_scale", "output", "x_q", "x_scale", "status")]
 
 
 class DispatchArgs(ctypes.Structure):
@@ -111,6 +130,11 @@ EXPORTS = {
     "b200moe_down": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "b200moe_combine": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "b200moe_route": (ctypes.c_int, [ctypes.POINTER(RouteArgs), ctypes.c_void_p]),
+    "b200moe_linear_create": (ctypes.c_int, [ctypes.POINTER(LinearShape), ctypes.POINTER(ctypes.c_void_p)]),
+    "b200moe_linear_workspace": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(LinearWorkspace)]),
+    "b200moe_linear_bind": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(LinearBuffers)]),
+    "b200moe_linear_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "b200moe_linear_destroy": (None, [ctypes.c_void_p]),
     "b200moe_dispatch_static": (ctypes.c_int, [ctypes.POINTER(DispatchArgs), ctypes.c_void_p]),
     "b200moe_plan_chain": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p),
                                           ctypes.POINTER(ctypes.c_int32)]),
@@ -168,7 +192,6 @@ def check(code: int):
 def launch(call, args, device):
     """``call(args, stream)`` on the current stream of device ``device``; ``args`` is a struct or a plan handle. Kept
     short: for one token the kernels behind it take less time than this function."""
-    import torch
     arg = ctypes.byref(args) if isinstance(args, ctypes.Structure) else args
     if torch._C._cuda_getDevice() == device:
         code = call(arg, torch._C._cuda_getCurrentRawStream(device))

@@ -37,7 +37,7 @@ def _bound_tensors(prepared):
              prepared.activated, prepared.down_output, prepared.status, prepared.scratch]
     if prepared.source_rows is not None:
         bound.append(prepared.source_rows)
-    return bound
+    return bound + prepared.int8_workspace()
 
 
 @torch.library.custom_op(_LIB_NAME, mutates_args=("ids", "routing_weights", "output", "workspace"),
@@ -96,3 +96,33 @@ def route(logits: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor,
 @route.register_fake
 def _(logits, bias, ids, routing_weights, score, groups, kept_groups, group_score, renormalize, scale):
     return None
+
+
+@torch.library.custom_op("b200moe::int8_linear", mutates_args=("output", "x_q", "x_scale", "status"), device_types="cuda")
+def int8_linear(plan: int, x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, output: torch.Tensor,
+                x_q: torch.Tensor, x_scale: torch.Tensor, status: torch.Tensor) -> None:
+    """One product of the prepared plan (``b200moe_linear_forward``) for tracers. The kernels use the addresses bound at
+    prepare time; where a tracer passes copies, values are copied in and out as for ``forward``."""
+    prepared = _LINEARS[plan]()
+    if x.shape[0] == 0:
+        return
+    if x.data_ptr() != prepared.x.data_ptr():
+        prepared.x.copy_(x)
+    _native.launch(prepared._call, prepared._plan, prepared._device)
+    for given, real in ((output, prepared.output), (x_q, prepared.x_q), (x_scale, prepared.x_scale),
+                        (status, prepared.status)):
+        if given.data_ptr() != real.data_ptr():
+            given.copy_(real)
+
+
+@int8_linear.register_fake
+def _(plan, x, weight, weight_scale, output, x_q, x_scale, status):
+    return None
+
+
+_LINEARS = {}   # plan address -> weak reference to the PreparedInt8Linear that owns it
+
+
+def register_linear(prepared):
+    key = prepared._plan.value
+    _LINEARS[key] = weakref.ref(prepared, lambda _ref, key=key: _LINEARS.pop(key, None))

@@ -4,6 +4,7 @@
 #include <cstdio>
 #include <cstring>
 #include <new>
+#include "int8.h"
 #include "plan.h"
 
 namespace b200moe {
@@ -23,8 +24,10 @@ int round_up(int v, int m) { return (v + m - 1) / m * m; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 bool is_w4(int format) { return format == B200MOE_WEIGHTS_W4G128; }
+bool is_int8(const B200MoeShape& s) { return s.gate_up_format == B200MOE_WEIGHTS_INT8; }   // both projections or neither
 
 bool tc_shape_ok(const B200MoeShape& s) {
+  if (is_int8(s)) return true;   // rows of int8 are padded to what TMA needs
   if (is_w4(s.gate_up_format) && s.hidden % 128) return false;    // one scale per 128 along K
   if (is_w4(s.down_format) && s.intermediate % 128) return false;
   return s.hidden % 8 == 0 && s.intermediate % 8 == 0 && s.hidden >= 64 && s.intermediate >= 64;
@@ -102,10 +105,110 @@ int encode_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, 
   return B200MOE_OK;
 }
 
+}  // namespace
+
+int encode_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows,
+              bool weights) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available from this driver");
+    return B200MOE_ERR_CUDA;
+  }
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {pitch};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        weights ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (int8) failed with CUresult %d (rows=%llu cols=%llu box_rows=%u)",
+              static_cast<int>(r), static_cast<unsigned long long>(rows), static_cast<unsigned long long>(cols), box_rows);
+    return B200MOE_ERR_CUDA;
+  }
+  return B200MOE_OK;
+}
+
+namespace {
+
 int check_cuda(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return B200MOE_OK;
   set_error("%s: %s", what, cudaGetErrorString(e));
   return B200MOE_ERR_CUDA;
+}
+
+// Persistent grid of an int8 product: at most the tiles there can be.
+int i8_grid(const B200MoePlan& p, int n_out, int tile_channels) {
+  const long long tiles = (static_cast<long long>((p.routes + p.token_tile - 1) / p.token_tile) + p.shape.experts - 1) *
+                          ((n_out + tile_channels - 1) / tile_channels);
+  return static_cast<int>(tiles < p.num_sms ? tiles : p.num_sms);
+}
+
+// Tensor maps and launch parameters of the two products of an INT8 plan.
+int bind_int8(B200MoePlan& p) {
+  const B200MoeShape& s = p.shape;
+  const B200MoeBuffers& b = p.buf;
+  int rc;
+  if ((rc = configure_i8())) return rc;
+  I8Gemm& gu = p.i8_gate_up;
+  I8Gemm& dn = p.i8_down;
+  gu = I8Gemm{};
+  gu.offsets = static_cast<const int*>(b.offsets);
+  gu.counts = static_cast<const int*>(b.counts);
+  gu.tasks = static_cast<const int*>(b.tasks);
+  gu.status = static_cast<int*>(b.status);
+  gu.groups = s.experts;
+  gu.rows = p.routes;
+  gu.token_tile = p.token_tile;
+  gu.stream_weights = static_cast<long long>(p.routes) <= static_cast<long long>(s.experts) * p.token_tile;
+  int smem = 0;
+  gu.stages = i8_stages(p.token_tile, &smem);
+  dn = gu;
+  gu.w_scale = static_cast<const float*>(b.gate_up_scales);
+  gu.row_scale = static_cast<const float*>(b.x_scale);
+  gu.out = b.activated;
+  gu.x_q = static_cast<const int8_t*>(b.x_q);
+  gu.source_rows = static_cast<const int*>(b.source_rows);
+  gu.n_out = s.intermediate;
+  gu.k = s.hidden;
+  gu.w_rows = 2 * s.intermediate;
+  dn.w_scale = static_cast<const float*>(b.down_scales);
+  dn.row_scale = static_cast<const float*>(b.activated_scale);
+  dn.out = b.down_output;
+  dn.n_out = s.hidden;
+  dn.k = s.intermediate;
+  dn.w_rows = s.hidden;
+  const uint64_t E = s.experts, I = s.intermediate, H = s.hidden;
+  if ((rc = encode_i8(&gu.tm_w, b.gate_up, E * 2 * I, H, int8_pitch(s.hidden), 128, true))) return rc;
+  if ((rc = encode_i8(&dn.tm_w, b.down, E * H, I, int8_pitch(s.intermediate), 128, true))) return rc;
+  return encode_i8(&dn.tm_act, b.activated_q, p.routes, I, int8_pitch(s.intermediate), p.token_tile, false);
+}
+
+int launch_int8_gate_up(const B200MoePlan& p, cudaStream_t s) {
+  QuantizeRows q{};
+  q.x = p.buf.x;
+  q.pitch = q.k = p.shape.hidden;
+  q.dtype = B200MOE_BF16;
+  q.rows = p.shape.tokens;
+  q.q = static_cast<int8_t*>(p.buf.x_q);
+  q.scale = static_cast<float*>(p.buf.x_scale);
+  cudaError_t e = launch_quantize_rows(q, s);
+  if (e == cudaSuccess) e = launch_i8_gate_up(p.i8_gate_up, p.gather, i8_grid(p, p.shape.intermediate, 128), s);
+  return check_cuda(e, "gate_up launch");
+}
+
+int launch_int8_down(const B200MoePlan& p, cudaStream_t s) {
+  QuantizeRows q{};
+  q.x = p.buf.activated;
+  q.pitch = q.k = p.shape.intermediate;
+  q.dtype = B200MOE_FP32;
+  q.rows = p.routes;
+  q.q = static_cast<int8_t*>(p.buf.activated_q);
+  q.scale = static_cast<float*>(p.buf.activated_scale);
+  cudaError_t e = launch_quantize_rows(q, s);
+  if (e == cudaSuccess) e = launch_i8_product(p.i8_down, B200MOE_BF16, i8_grid(p, p.shape.hidden, 256), s);
+  return check_cuda(e, "down launch");
 }
 
 int require_bound(const B200MoePlan* p) {
@@ -165,9 +268,23 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
     return B200MOE_ERR_UNSUPPORTED;
   }
   for (int f : {s.gate_up_format, s.down_format}) {
-    if (f != B200MOE_WEIGHTS_BF16 && f != B200MOE_WEIGHTS_W4G128) {
+    if (f != B200MOE_WEIGHTS_BF16 && f != B200MOE_WEIGHTS_W4G128 && f != B200MOE_WEIGHTS_INT8) {
       set_error("unknown weight format %d", f);
       return B200MOE_ERR_INVALID;
+    }
+  }
+  if ((s.gate_up_format == B200MOE_WEIGHTS_INT8) != (s.down_format == B200MOE_WEIGHTS_INT8)) {
+    set_error("INT8 weights: both projections take this format or neither does");
+    return B200MOE_ERR_INVALID;
+  }
+  if (is_int8(s)) {
+    if (s.hidden > kInt8MaxK || s.intermediate > kInt8MaxK) {
+      set_error("INT8 weights: H and I are at most %d (32-bit sums; H=%d I=%d)", kInt8MaxK, s.hidden, s.intermediate);
+      return B200MOE_ERR_INVALID;
+    }
+    if (s.schedule == B200MOE_SCHEDULE_GENERIC || s.route_only || s.external_dispatch) {
+      set_error("INT8 weights run on the tcgen05 schedule of an ordinary plan (no expert-parallel halves)");
+      return B200MOE_ERR_UNSUPPORTED;
     }
   }
   const bool any_w4 = is_w4(s.gate_up_format) || is_w4(s.down_format);
@@ -248,7 +365,8 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   // against 330.3 / 508.0 / 871.7 us): there the activated rows are still in L2 and sharing them between two
   // channel tiles, which is what pair tiles do, is worth as much.
   p->down_tile = tile;
-  if (schedule == B200MOE_SCHEDULE_TCGEN05 && !is_w4(s.down_format) && !s.route_only) {
+  if (schedule == B200MOE_SCHEDULE_TCGEN05 && !is_w4(s.down_format) && !is_int8(s) &&
+      !s.route_only) {
     if (s.down_tiles == 3 && tile != 128) {
       delete p;
       set_error("down_tiles = 3 (wide tiles) needs token tile 128 (resolved token tile: %d)", tile);
@@ -271,6 +389,7 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   p->gather = s.fused_gather && schedule == B200MOE_SCHEDULE_TCGEN05 && !s.route_only && !s.external_dispatch &&
               r > 0 && (!is_w4(s.gate_up_format) || tile <= 16) &&
               (s.fused_gather == 2 || r <= static_cast<long long>(s.experts) * 384);
+  if (is_int8(s)) p->gather = r > 0;   // there are no BF16 rows to group: the quantised ones are gathered at any size
 
   B200MoeWorkspace& w = p->ws;
   const size_t T = s.tokens, H = s.hidden, I = s.intermediate, E = s.experts, R = r;
@@ -282,17 +401,24 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   w.mapping = R * 4;
   w.ranks = R * 4;
   w.grouped_input = R * H * 2;
-  w.activated = s.route_only ? 0 : R * I * 2;
+  w.activated = s.route_only ? 0 : R * I * (is_int8(s) ? 4 : 2);
   w.down_output = R * H * 2;
   w.status = 4;
   w.scratch = align256((static_cast<size_t>(p->partitions) * E + blocks + 2 + E) * 4);
   w.source_rows = p->gather ? R * 4 : 0;
+  if (is_int8(s)) {
+    w.x_q = T * int8_pitch(s.hidden);
+    w.x_scale = T * 4;
+    w.activated_q = R * int8_pitch(s.intermediate);
+    w.activated_scale = R * 4;
+  }
   w.gathers = p->gather ? 1 : 0;
   w.down_tiles = p->down_tiles;
   if (p->gather) w.grouped_input = 0;
   w.token_tile = tile;
   w.schedule = schedule;
   w.launches = s.tokens == 0 ? 0 : (s.use_router ? 1 : 0) + (p->dispatch_fused ? 2 : 3) + (s.route_only ? 0 : 3);
+  if (is_int8(s) && s.tokens) w.launches += 2;       // x and the activated rows are quantised
   if (s.route_only == 2) w.launches -= 1;            // no row copy
   if (p->gather && p->dispatch_fused) w.launches -= 1;  // no row copy kernel
   if (s.external_dispatch) w.launches = s.tokens == 0 ? 0 : 2;  // gate_up + down only
@@ -356,6 +482,16 @@ int b200moe_plan_bind(B200MoePlan* p, const B200MoeBuffers* b) {
         if (!check(n)) return B200MOE_ERR_INVALID;
     if (s.route_only != 2 && !p->gather && !check({b->grouped_input, "grouped_input"})) return B200MOE_ERR_INVALID;
     if (p->gather && !check({b->source_rows, "source_rows"})) return B200MOE_ERR_INVALID;
+    if (is_int8(s)) {
+      for (const Named& n : {Named{b->x_q, "x_q"}, Named{b->x_scale, "x_scale"}, Named{b->activated_q, "activated_q"},
+                             Named{b->activated_scale, "activated_scale"}, Named{b->gate_up_scales, "gate_up_scales"},
+                             Named{b->down_scales, "down_scales"}})
+        if (!check(n)) return B200MOE_ERR_INVALID;
+      if ((reinterpret_cast<uintptr_t>(b->x_q) | reinterpret_cast<uintptr_t>(b->activated_q)) % 16) {
+        set_error("INT8 plan: x_q and activated_q must be 16-byte aligned");
+        return B200MOE_ERR_INVALID;
+      }
+    }
     if (!s.external_dispatch && s.ids_are_int64 && reinterpret_cast<uintptr_t>(b->ids) % 8) {
       set_error("buffer 'ids' (int64) is not 8-byte aligned");
       return B200MOE_ERR_INVALID;
@@ -370,7 +506,8 @@ int b200moe_plan_bind(B200MoePlan* p, const B200MoeBuffers* b) {
     }
     // the output and the workspace must not alias the inputs (cuda_gate_up.cu:150-158)
     const void* inputs[] = {b->x, b->gate_up, b->down, b->ids, b->routing_weights, b->router_weight, b->residual};
-    const void* written[] = {b->output, b->grouped_input, b->activated, b->down_output, b->mapping, b->ranks};
+    const void* written[] = {b->output, b->grouped_input, b->activated, b->down_output, b->mapping, b->ranks,
+                             b->x_q, b->activated_q};
     for (const void* in : inputs)
       for (const void* wr : written)
         if (in && in == wr) {
@@ -392,7 +529,7 @@ int b200moe_plan_bind(B200MoePlan* p, const B200MoeBuffers* b) {
   }
   p->buf = *b;
   p->router_tc = false;
-  if (s.tokens > 0 && s.use_router && p->schedule == B200MOE_SCHEDULE_TCGEN05 &&
+  if (s.tokens > 0 && s.use_router && p->schedule == B200MOE_SCHEDULE_TCGEN05 && s.hidden % 8 == 0 && s.hidden >= 64 &&
       (reinterpret_cast<uintptr_t>(b->x) | reinterpret_cast<uintptr_t>(b->router_weight)) % 16 == 0) {
     const uint32_t e_pad = static_cast<uint32_t>((s.experts + 15) / 16 * 16);
     if ((rc = encode_2d(&p->tm_x, b->x, s.tokens, s.hidden, 128, false))) return rc;
@@ -406,13 +543,19 @@ int b200moe_plan_bind(B200MoePlan* p, const B200MoeBuffers* b) {
     }
   }
   if (s.tokens > 0 && p->schedule == B200MOE_SCHEDULE_TCGEN05 && !s.route_only) {
-    const void* aligned16[] = {b->gate_up, b->down, p->gather ? b->x : b->grouped_input, b->activated};
+    const void* rows16 = is_int8(s) ? b->x_q : p->gather ? b->x : b->grouped_input;
+    const void* aligned16[] = {b->gate_up, b->down, rows16, b->activated};
     for (const void* ptr : aligned16)
       if (reinterpret_cast<uintptr_t>(ptr) % 16) {
         set_error("tcgen05 schedule: weights and workspace rows must be 16-byte aligned");
         return B200MOE_ERR_INVALID;
       }
     const uint64_t E = s.experts, H = s.hidden, I = s.intermediate, R = p->routes;
+    if (is_int8(s)) {
+      if ((rc = bind_int8(*p))) return rc;
+      p->bound = true;
+      return B200MOE_OK;
+    }
     if (is_w4(s.gate_up_format)) {
       if (!b->gate_up_scales) {
         set_error("W4G128 gate/up needs gate_up_scales");
@@ -464,6 +607,7 @@ int b200moe_dispatch(B200MoePlan* p, void* stream) {
 // Inside b200moe_forward the two BF16 tensor-core GEMMs are chained through per-expert counters.
 static bool w4_in_tmem(const B200MoePlan* p) { return p->token_tile <= 64; }
 static bool chain_stages(const B200MoePlan* p) {
+  if (is_int8(p->shape)) return false;
   if (p->shape.unchained || p->schedule != B200MOE_SCHEDULE_TCGEN05 || p->shape.external_dispatch == 1 || !p->buf.scratch)
     return false;
   const bool g4 = is_w4(p->shape.gate_up_format), d4 = is_w4(p->shape.down_format);
@@ -486,6 +630,7 @@ static int gate_up_stage(B200MoePlan* p, void* stream, bool chained) {
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->schedule != B200MOE_SCHEDULE_TCGEN05) return check_cuda(launch_gate_up_generic(*p, s), "gate_up launch");
+  if (is_int8(p->shape)) return launch_int8_gate_up(*p, s);
   // W4: up to 16 rows per tile the weights are dequantised in registers (weight-streaming kernel); above, the
   // dequantised operand goes to tensor memory while two accumulator sets still fit beside it (tile <= 64), to
   // shared memory above that
@@ -506,6 +651,7 @@ static int down_stage(B200MoePlan* p, void* stream, bool chained) {
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->schedule != B200MOE_SCHEDULE_TCGEN05) return check_cuda(launch_down_generic(*p, s), "down launch");
+  if (is_int8(p->shape)) return launch_int8_down(*p, s);
   if (is_w4(p->shape.down_format)) {
     if (w4r_serves(*p)) return check_cuda(launch_down_w4r(*p, s, chained), "down launch");
     return check_cuda(w4_in_tmem(p) ? launch_down_w4t(*p, s, chained) : launch_down_w4(*p, s, chained), "down launch");

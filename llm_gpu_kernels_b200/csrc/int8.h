@@ -1,0 +1,50 @@
+// The 8-bit integer kernels behind INT8 plans (abi.cu) and the dense product (linear.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+#include "../../include/b200moe.h"
+
+namespace b200moe {
+
+constexpr int kInt8MaxK = 131072;   // 127 * 127 * K stays below 2^31
+
+constexpr int int8_pitch(int k) { return (k + 15) / 16 * 16; }   // bytes of a row of int8: TMA strides are multiples of 16
+
+struct QuantizeRows {
+  const void* x;
+  long long pitch;   // elements
+  int dtype;         // B200MOE_BF16 / FP16 / FP32
+  int rows, k;
+  int8_t* q;         // [rows, int8_pitch(k)]
+  float* scale;      // [rows]
+};
+cudaError_t launch_quantize_rows(const QuantizeRows& a, cudaStream_t s);
+
+// One grouped product in int8 (grouped_gemm_i8.cu). Rows of group e are offsets[e] .. + counts[e] of the activations, or
+// without `tasks` all `rows` of them belong to the one group there is.
+struct I8Gemm {
+  CUtensorMap tm_w;            // int8 [groups * w_rows, k], rows int8_pitch(k) bytes apart, box 128 bytes x 128 rows
+  CUtensorMap tm_act;          // int8 [rows, k], box 128 bytes x token_tile rows (not read when gathering)
+  const float* w_scale;        // [groups * w_rows]
+  const float* row_scale;      // [rows]; gathering: [tokens]
+  void* out;                   // gate/up: float [rows, n_out]; else [rows, n_out] of out_dtype
+  const int* offsets;
+  const int* counts;
+  const int* tasks;
+  int* status;
+  const int8_t* x_q;           // gathering: [tokens, int8_pitch(k)]
+  const int* source_rows;      // gathering: token of each row
+  const unsigned char* prefetch_base;
+  int prefetch_chunks;
+  int groups, rows, n_out, k, w_rows, token_tile, stages, stream_weights;
+};
+int i8_stages(int token_tile, int* smem_bytes);
+int configure_i8();   // opt-in shared memory of the kernels on the current device
+cudaError_t launch_i8_gate_up(const I8Gemm& g, bool gather, int grid, cudaStream_t s);
+cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, int grid, cudaStream_t s);
+// 2-D int8 tensor map, box 128 bytes x box_rows, 128-byte swizzle, zero fill past the ends.
+int encode_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows,
+              bool weights);
+
+}  // namespace b200moe

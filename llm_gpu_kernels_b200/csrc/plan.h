@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 #include "../../include/b200moe.h"
+#include "int8.h"
 #include "route_row.cuh"
 
 struct B200MoePlan {
@@ -48,6 +49,8 @@ struct B200MoePlan {
   // the weight-streaming W4A16 kernel (token tile <= 16): dequantisation in registers, mma.sync
   int w4r_stages_gate_up = 0, w4r_smem_gate_up = 0;
   int w4r_stages_down = 0, w4r_smem_down = 0;
+  // INT8 plans: the two products
+  b200moe::I8Gemm i8_gate_up{}, i8_down{};
 };
 
 namespace b200moe {

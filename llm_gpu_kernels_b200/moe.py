@@ -23,6 +23,7 @@ import torch
 
 from . import _native, _ops
 from .gemm import GemmConfig
+from .int8_weights import Int8Weight
 from .moe_router import RouterConfig, check_bias
 
 STAGE_NAMES = ("router", "dispatch", "gate_up_swiglu", "down", "combine")
@@ -100,6 +101,10 @@ class PreparedMoE:
     down_tiles: int = 0       # resolved BF16 down schedule: 1 pair, 2 128-channel tiles (two partial sums), 3 wide
                               # (256-row tiles); pass it as ``down_tiles=`` to a plan that must give the same bits
     source_rows: torch.Tensor = None   # [R] int32: the token behind each grouped row (only when gathers)
+    x_q: torch.Tensor = None             # INT8 plans: quantised rows and their scales, rewritten by every run
+    x_scale: torch.Tensor = None
+    activated_q: torch.Tensor = None
+    activated_scale: torch.Tensor = None
     fused_return: bool = False  # expert-side plans: the down projection stores result rows into their owners' buffers
     ep_tables: tuple = None
     _plan: object = field(default=None, repr=False)
@@ -112,7 +117,12 @@ class PreparedMoE:
         return sum(t.numel() * t.element_size() for t in
                    (self.counts, self.offsets, self.cursors, self.tasks, self.mapping, self.grouped_input,
                     self.projected, self.activated, self.down_output, self.status, self.scratch)
-                   ) + (self.source_rows.numel() * 4 if self.source_rows is not None else 0)
+                   ) + sum(t.numel() * t.element_size() for t in self.int8_workspace()
+                           ) + (self.source_rows.numel() * 4 if self.source_rows is not None else 0)
+
+    def int8_workspace(self):
+        """The tensors only INT8 plans have."""
+        return [t for t in (self.x_q, self.x_scale, self.activated_q, self.activated_scale) if t is not None]
 
     def check_inputs(self):
         flags = int(self.status.item())
@@ -151,13 +161,15 @@ class PreparedMoE:
         if self.x.shape[0] == 0:
             return self.output
         if self._op_args is None:
-            weights = [t for t in (self.gate_up, self.down, self.router_weight, self.gate_up_scales,
+            weights = [t.storage if isinstance(t, Int8Weight) else t for t in (self.gate_up, self.down)]
+            weights = [t for t in (*weights, self.router_weight, self.gate_up_scales,
                                    self.down_scales, self.valid_routes, self.residual, self.router_bias)
                        if t is not None]
             workspace = [self.counts, self.offsets, self.cursors, self.tasks, self.mapping, self.ranks,
                          self.grouped_input, self.activated, self.down_output, self.status, self.scratch]
             if self.source_rows is not None:
                 workspace.append(self.source_rows)
+            workspace += self.int8_workspace()
             self._op_args = (self._plan.value, self.x, weights, self.ids, self.routing_weights, self.output, workspace)
             _ops.register_plan(self)
         _ops.forward(*self._op_args)
@@ -191,13 +203,16 @@ def _validate(x, gate_up, down, ids, routing_weights, router_weight, gate_up_sca
         e, h, intermediate = int(route_only_experts), x.shape[1], 64
         gate_up_shape = (e, 2 * intermediate, h)
         gate_up = down = None
+    elif isinstance(gate_up, Int8Weight):
+        gate_up_shape = tuple(gate_up.shape)
+        e, h, intermediate = down.shape
     elif gate_up_scales is None:
         _input(gate_up, 3)
         gate_up_shape = tuple(gate_up.shape)
     else:
         _packed_input(gate_up, gate_up_scales, "gate_up")
         gate_up_shape = (gate_up.shape[0], gate_up.shape[1], gate_up.shape[2] * 8)
-    if route_only_experts is not None:
+    if route_only_experts is not None or isinstance(gate_up, Int8Weight):
         pass
     elif down_scales is None:
         _input(down, 3)
@@ -214,7 +229,8 @@ def _validate(x, gate_up, down, ids, routing_weights, router_weight, gate_up_sca
             or routing_weights.dtype != torch.float32):
         raise ValueError("expected CUDA IDs[T,topk<=32] and FP32 weights of identical shape")
     extra = [t for t in (gate_up_scales, down_scales) if t is not None]
-    weights = [t for t in (gate_up, down) if t is not None]
+    weights = [t.storage if isinstance(t, Int8Weight) else t for t in (gate_up, down) if t is not None]
+    weights += [t.scales for t in (gate_up, down) if isinstance(t, Int8Weight)]
     if any(t.device != x.device or not t.is_contiguous() for t in (*weights, ids, routing_weights, *extra)):
         raise ValueError("all MoE tensors must be contiguous and on the same CUDA device")
     r = ids.numel()
@@ -265,12 +281,14 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
                                  or residual.device != x.device or not residual.is_contiguous()):
         raise ValueError("residual must be a contiguous bfloat16 tensor of the shape and device of x")
     lib = _native.load()
+    int8 = isinstance(gate_up, Int8Weight)
     tokens = x.shape[0]
     topk = ids.shape[1]
+    weight_format = lambda scales: (_native.WEIGHTS_INT8 if int8 else _native.WEIGHTS_BF16 if scales is None
+                                    else _native.WEIGHTS_W4G128)
     shape = _native.Shape(tokens=tokens, experts=e, topk=topk, hidden=h, intermediate=intermediate,
                           ids_are_int64=int(ids.dtype == torch.int64),
-                          gate_up_format=_native.WEIGHTS_BF16 if gate_up_scales is None else _native.WEIGHTS_W4G128,
-                          down_format=_native.WEIGHTS_BF16 if down_scales is None else _native.WEIGHTS_W4G128,
+                          gate_up_format=weight_format(gate_up_scales), down_format=weight_format(down_scales),
                           schedule=_SCHEDULES[schedule], token_tile=int(token_tile),
                           use_router=0 if router_weight is None else 1 if router is None else 2,
                           router=router.native() if router is not None else _native.RouterConfig(),
@@ -293,7 +311,8 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             x, gate_up, down, ids, routing_weights, bf16((tokens, h)),
             int32((e,)), int32((e,)), int32((e,)), int32((e + 1,)), int32((r,)),
             bf16((0 if sizes.gathers else r, h)), bf16((0, 2 * intermediate)),
-            bf16((0 if route_only_experts is not None else r, intermediate)), bf16((r, h)),
+            torch.empty((0 if route_only_experts is not None else r, intermediate), device=device,
+                        dtype=torch.float32 if int8 else torch.bfloat16), bf16((r, h)),
             int32((1,)), config,
             ranks=int32((r,)), scratch=int32((max(1, sizes.scratch // 4),)), router_weight=router_weight,
             router=router, router_bias=router_bias, schedule=_native.SCHEDULE_NAMES[sizes.schedule], token_tile=sizes.token_tile,
@@ -301,6 +320,11 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             valid_routes=valid_routes, residual=residual, gathers=bool(sizes.gathers), down_pair=sizes.down_tiles == 1,
             down_tiles=sizes.down_tiles,
             source_rows=int32((r,)) if sizes.gathers else None)
+        if int8:
+            byte = lambda rows, size: torch.empty((rows, size // max(1, rows)), device=device, dtype=torch.int8)
+            plan.x_q, plan.activated_q = byte(tokens, sizes.x_q), byte(r, sizes.activated_q)
+            plan.x_scale = torch.empty((tokens,), device=device, dtype=torch.float32)
+            plan.activated_scale = torch.empty((r,), device=device, dtype=torch.float32)
         for name, tensor in (workspace or {}).items():  # caller-provided workspace (peer-visible buffers)
             if tuple(tensor.shape) != tuple(getattr(plan, name).shape) or tensor.dtype != getattr(plan, name).dtype:
                 raise ValueError(f"workspace override {name} has the wrong shape or dtype")
@@ -309,15 +333,19 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
                     "cursors": plan.cursors, "tasks": plan.tasks, "mapping": plan.mapping, "ranks": plan.ranks,
                     "grouped_input": plan.grouped_input, "activated": plan.activated,
                     "down_output": plan.down_output, "status": plan.status, "scratch": plan.scratch}
+        if int8:
+            expected.update({name: getattr(plan, name) for name in _native.INT8_BUFFERS})
+            gate_up_scales, down_scales = gate_up.scales, down.scales
         for name, tensor in expected.items():
             if tensor.numel() * tensor.element_size() < getattr(sizes, name):
                 raise RuntimeError(f"workspace buffer {name} smaller than the library requires")
         if sizes.gathers and plan.source_rows.numel() * 4 < sizes.source_rows:
             raise RuntimeError("workspace buffer source_rows smaller than the library requires")
         ptr = lambda t: ctypes.c_void_p(t.data_ptr()) if t is not None and t.numel() else None
+        stored = lambda t: t.storage if isinstance(t, Int8Weight) else t
         buffers = _native.Buffers(
-            x=ptr(x), router_weight=ptr(router_weight), gate_up=ptr(gate_up), gate_up_scales=ptr(gate_up_scales),
-            down=ptr(down), down_scales=ptr(down_scales), ids=ptr(ids), routing_weights=ptr(routing_weights),
+            x=ptr(x), router_weight=ptr(router_weight), gate_up=ptr(stored(gate_up)), gate_up_scales=ptr(gate_up_scales),
+            down=ptr(stored(down)), down_scales=ptr(down_scales), ids=ptr(ids), routing_weights=ptr(routing_weights),
             valid_routes=ptr(valid_routes), residual=ptr(residual), source_rows=ptr(plan.source_rows),
             router_bias=ptr(router_bias),
             **{name: ptr(tensor) for name, tensor in expected.items()})
