@@ -21,6 +21,18 @@ struct QuantizeRows {
 };
 cudaError_t launch_quantize_rows(const QuantizeRows& a, cudaStream_t s);
 
+// The dense product for a few tokens (linear_small.cu), which quantises x itself.
+struct LinearSmall {
+  const void* x;
+  long long x_pitch;   // elements
+  const int8_t* weight;
+  const float* w_scale;
+  void* y;
+  int dtype, tokens, k, n, sms;
+};
+bool linear_small_serves(int tokens, int k);
+cudaError_t launch_linear_small(const LinearSmall& a, cudaStream_t s);
+
 // One grouped product in int8 (grouped_gemm_i8.cu). Rows of group e are offsets[e] .. + counts[e] of the activations, or
 // without `tasks` all `rows` of them belong to the one group there is.
 struct I8Gemm {

@@ -1,67 +1,17 @@
-// Rows to 8-bit integers, one scale per row:
-//   top = max |x_k|,  q_k = rint(127 x_k / top)  (ties to even),  scale = top / 127
-// A row of zeros gives zeros and scale 0; a row that holds an infinity or a NaN gives zeros and scale NaN, so every
-// product of it is NaN. q is that of exact arithmetic on the values read: x * (127 / top) in FP32 is off by at most
-// 2^-16 (two roundings of values up to 127), so only a quotient that close to a half may round the wrong way, and
-// those few are divided again in FP64 (where a 16-bit or 24-bit x over top cannot come closer to a half without being
-// one than 2^-33).
+// Rows to 8-bit integers in memory (the formula and its rounding: int8_rows.cuh).
 // Bound by memory: it reads a row once (up to 32 values per thread stay in registers between the maximum and the
 // rounding) and writes a byte per value; at a serving batch by launch latency.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include "int8.h"
+#include "int8_rows.cuh"
 #include "pdl.cuh"
 
 namespace b200moe {
 namespace {
 
+using namespace rows8;
+
 constexpr int kThreads = 256;
 constexpr int kCached = 4;   // pieces of 8 values a thread keeps
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-
-// Values k .. k+7 of a row, zero past its end.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int k, int K, float (&v)[8]) {
-  if (kVec) {
-    union { T t[8]; uint4 q[sizeof(T) / 2]; } raw;
-    if (k < K) {   // K is a multiple of 8 here
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw.q[i] = *(reinterpret_cast<const uint4*>(row + k) + i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_float(raw.t[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_float(row[k + j]) : 0.0f;
-  }
-}
-
-__device__ __forceinline__ uint32_t top_bits(const float (&v)[8], uint32_t top) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);   // NaN > Inf > finite
-  return top;
-}
-
-// up: a power of two that lifts the row out of the subnormal range.
-__device__ __forceinline__ int round_to_int8(float x, float inverse, float top, float up) {
-  const float t = x * up * inverse, r = rintf(t);
-  if (fabsf(t - r) > 0.4999f) return static_cast<int>(rint(127.0 * static_cast<double>(x) * up / static_cast<double>(top)));
-  return static_cast<int>(r);
-}
-
-__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inverse, float top, float up) {
-  uint32_t w[2] = {0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    w[j >> 2] |= (static_cast<uint32_t>(round_to_int8(v[j], inverse, top, up)) & 0xffu) << (8 * (j & 3));
-  return make_uint2(w[0], w[1]);
-}
 
 // L threads per row (a power of two, 32 .. 256).
 template <typename T, int L, bool kVec>
@@ -96,23 +46,18 @@ quantize_rows_kernel(const T* __restrict__ x, long long pitch, int8_t* __restric
     for (int w = 0; w < L / 32; ++w) bits = max(bits, part[first + w]);
   }
   if (!live) return;
-  const bool finite = bits < 0x7f800000u;
-  float top = __uint_as_float(bits);
-  if (t == 0) scale[row] = finite ? top / 127.0f : __uint_as_float(0x7fffffffu);
-  const float up = top < 1e-30f ? 0x1p100f : 1.0f;
-  top *= up;
-  const bool zero = !finite || bits == 0;
-  const float inverse = zero ? 0.0f : 127.0f / top;
+  const RowScale r = row_scale_of(bits);
+  if (t == 0) scale[row] = r.scale;
   int8_t* dst = q + static_cast<size_t>(row) * q_pitch;
 #pragma unroll
   for (int c = 0; c < kCached; ++c) {
     const int k = (c * L + t) * 8;
-    if (k < q_pitch) *reinterpret_cast<uint2*>(dst + k) = zero ? make_uint2(0u, 0u) : quantize8(v[c], inverse, top, up);
+    if (k < q_pitch) *reinterpret_cast<uint2*>(dst + k) = quantize8(v[c], r);
   }
   for (int k = (kCached * L + t) * 8; k < q_pitch; k += L * 8) {
     float u[8];
     load8<T, kVec>(src, k, K, u);
-    *reinterpret_cast<uint2*>(dst + k) = zero ? make_uint2(0u, 0u) : quantize8(u, inverse, top, up);
+    *reinterpret_cast<uint2*>(dst + k) = quantize8(u, r);
   }
 }
 

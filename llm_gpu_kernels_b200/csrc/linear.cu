@@ -8,7 +8,8 @@ struct B200MoeLinear {
   B200MoeLinearShape shape{};
   B200MoeLinearBuffers buf{};
   bool bound = false;
-  int token_tile = 0, grid = 0;
+  bool small = false;   // a few tokens: one kernel without tensor cores
+  int token_tile = 0, grid = 0, sms = 0;
   b200moe::I8Gemm gemm{};
 };
 
@@ -52,6 +53,7 @@ int b200moe_linear_create(const B200MoeLinearShape* shape, B200MoeLinear** out) 
     return B200MOE_ERR_INVALID;
   }
   p->shape = *shape;
+  p->small = linear_small_serves(shape->tokens, shape->k);
   p->token_tile = token_tile_of(shape->tokens);
   *out = p;
   return B200MOE_OK;
@@ -66,7 +68,7 @@ int b200moe_linear_workspace(const B200MoeLinear* p, B200MoeLinearWorkspace* w) 
   w->x_q = static_cast<size_t>(p->shape.tokens) * int8_pitch(p->shape.k);
   w->x_scale = static_cast<size_t>(p->shape.tokens) * 4;
   w->status = 4;
-  w->launches = p->shape.tokens ? 2 : 0;
+  w->launches = p->shape.tokens == 0 ? 0 : p->small ? 1 : 2;
   return B200MOE_OK;
 }
 
@@ -111,6 +113,11 @@ int b200moe_linear_bind(B200MoeLinear* p, const B200MoeLinearBuffers* b) {
     set_error("this library is built for sm_100a only; device %d has compute capability major %d", device, major);
     return B200MOE_ERR_UNSUPPORTED;
   }
+  p->sms = sms;
+  if (p->small) {
+    p->bound = true;
+    return B200MOE_OK;
+  }
   int rc;
   if ((rc = configure_i8())) return rc;
   I8Gemm& g = p->gemm;
@@ -147,6 +154,17 @@ int b200moe_linear_forward(B200MoeLinear* p, void* cuda_stream) {
   }
   if (p->shape.tokens == 0) return B200MOE_OK;
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (p->small) {
+    const LinearSmall a{p->buf.x, p->shape.tokens > 1 ? p->buf.x_pitch : p->shape.k, static_cast<const int8_t*>(p->buf.weight),
+                        static_cast<const float*>(p->buf.weight_scale), p->buf.output, p->shape.dtype, p->shape.tokens,
+                        p->shape.k, p->shape.n, p->sms};
+    const cudaError_t e = launch_linear_small(a, s);
+    if (e != cudaSuccess) {
+      set_error("linear launch: %s", cudaGetErrorString(e));
+      return B200MOE_ERR_CUDA;
+    }
+    return B200MOE_OK;
+  }
   QuantizeRows q{};
   q.x = p->buf.x;
   q.pitch = p->shape.tokens > 1 ? p->buf.x_pitch : p->shape.k;

@@ -155,9 +155,8 @@ class PreparedMoE:
         self._stage(4)
 
     def run(self):
-        """One forward on the current stream, through the registered PyTorch operator
-        ``torch.ops.b200moe.forward`` (a thin wrapper of ``b200moe_forward``), so that graph capture and
-        ``torch.compile`` see which tensors the call writes."""
+        """One forward on the current stream (``b200moe_forward``). While ``torch.compile`` traces, the call goes through
+        the registered PyTorch operator ``torch.ops.b200moe.forward``, which tells the tracer what it writes."""
         if self.x.shape[0] == 0:
             return self.output
         if self._op_args is None:
@@ -172,7 +171,11 @@ class PreparedMoE:
             workspace += self.int8_workspace()
             self._op_args = (self._plan.value, self.x, weights, self.ids, self.routing_weights, self.output, workspace)
             _ops.register_plan(self)
-        _ops.forward(*self._op_args)
+        if torch.compiler.is_compiling():
+            _ops.forward(*self._op_args)
+        else:
+            # the same call without the operator's dispatch, which takes longer than a small forward
+            _native.launch(self._forward, self._plan, self.x.device.index)
         return self.output
 
     def __del__(self):
