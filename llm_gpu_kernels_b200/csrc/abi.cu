@@ -138,13 +138,6 @@ int check_cuda(cudaError_t e, const char* what) {
   return B200MOE_ERR_CUDA;
 }
 
-// Persistent grid of an int8 product: at most the tiles there can be.
-int i8_grid(const B200MoePlan& p, int n_out, int tile_channels) {
-  const long long tiles = (static_cast<long long>((p.routes + p.token_tile - 1) / p.token_tile) + p.shape.experts - 1) *
-                          ((n_out + tile_channels - 1) / tile_channels);
-  return static_cast<int>(tiles < p.num_sms ? tiles : p.num_sms);
-}
-
 // Tensor maps and launch parameters of the two products of an INT8 plan.
 int bind_int8(B200MoePlan& p) {
   const B200MoeShape& s = p.shape;
@@ -162,14 +155,17 @@ int bind_int8(B200MoePlan& p) {
   gu.rows = p.routes;
   gu.token_tile = p.token_tile;
   gu.stream_weights = static_cast<long long>(p.routes) <= static_cast<long long>(s.experts) * p.token_tile;
+  gu.boxes = 2;
+  gu.split = 1;
+  gu.grid = p.num_sms;
   int smem = 0;
-  gu.stages = i8_stages(p.token_tile, &smem);
+  gu.stages = i8_stages(gu.boxes, p.token_tile, gu.split, &smem);
   dn = gu;
   gu.w_scale = static_cast<const float*>(b.gate_up_scales);
   gu.row_scale = static_cast<const float*>(b.x_scale);
   gu.out = b.activated;
   gu.x_q = static_cast<const int8_t*>(b.x_q);
-  gu.source_rows = static_cast<const int*>(b.source_rows);
+  gu.source_rows = p.gather ? static_cast<const int*>(b.source_rows) : nullptr;
   gu.n_out = s.intermediate;
   gu.k = s.hidden;
   gu.w_rows = 2 * s.intermediate;
@@ -181,6 +177,7 @@ int bind_int8(B200MoePlan& p) {
   dn.w_rows = s.hidden;
   const uint64_t E = s.experts, I = s.intermediate, H = s.hidden;
   if ((rc = encode_i8(&gu.tm_w, b.gate_up, E * 2 * I, H, int8_pitch(s.hidden), 128, true))) return rc;
+  if (!p.gather && (rc = encode_i8(&gu.tm_act, b.x_q, p.routes, H, int8_pitch(s.hidden), p.token_tile, false))) return rc;
   if ((rc = encode_i8(&dn.tm_w, b.down, E * H, I, int8_pitch(s.intermediate), 128, true))) return rc;
   return encode_i8(&dn.tm_act, b.activated_q, p.routes, I, int8_pitch(s.intermediate), p.token_tile, false);
 }
@@ -193,8 +190,12 @@ int launch_int8_gate_up(const B200MoePlan& p, cudaStream_t s) {
   q.rows = p.shape.tokens;
   q.q = static_cast<int8_t*>(p.buf.x_q);
   q.scale = static_cast<float*>(p.buf.x_scale);
+  if (!p.gather) {   // straight into grouped order
+    q.mapping = static_cast<const int*>(p.buf.mapping);
+    q.copies = p.shape.topk;
+  }
   cudaError_t e = launch_quantize_rows(q, s);
-  if (e == cudaSuccess) e = launch_i8_gate_up(p.i8_gate_up, p.gather, i8_grid(p, p.shape.intermediate, 128), s);
+  if (e == cudaSuccess) e = launch_i8_gate_up(p.i8_gate_up, s);
   return check_cuda(e, "gate_up launch");
 }
 
@@ -207,7 +208,7 @@ int launch_int8_down(const B200MoePlan& p, cudaStream_t s) {
   q.q = static_cast<int8_t*>(p.buf.activated_q);
   q.scale = static_cast<float*>(p.buf.activated_scale);
   cudaError_t e = launch_quantize_rows(q, s);
-  if (e == cudaSuccess) e = launch_i8_product(p.i8_down, B200MOE_BF16, i8_grid(p, p.shape.hidden, 256), s);
+  if (e == cudaSuccess) e = launch_i8_product(p.i8_down, B200MOE_BF16, s);
   return check_cuda(e, "down launch");
 }
 
@@ -329,6 +330,7 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   p->routes = static_cast<int>(r);
   p->schedule = schedule;
   p->token_tile = tile;
+  p->int8 = is_int8(s);
   p->dispatch_fused = r <= static_cast<long long>(kFusedRoutes) * kFusedCluster;
   if (p->dispatch_fused) {  // the 32 warps of each block of a cluster share the routes
     p->dispatch_ctas = 1;   // 1, 2, 4 or 8
@@ -389,7 +391,9 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   p->gather = s.fused_gather && schedule == B200MOE_SCHEDULE_TCGEN05 && !s.route_only && !s.external_dispatch &&
               r > 0 && (!is_w4(s.gate_up_format) || tile <= 16) &&
               (s.fused_gather == 2 || r <= static_cast<long long>(s.experts) * 384);
-  if (is_int8(s)) p->gather = r > 0;   // there are no BF16 rows to group: the quantised ones are gathered at any size
+  // INT8: no BF16 rows are grouped. The quantised rows are gathered, or past the same three tiles per expert written in
+  // grouped order by the kernel that quantises them.
+  if (is_int8(s)) p->gather = r > 0 && r <= static_cast<long long>(s.experts) * 384;
 
   B200MoeWorkspace& w = p->ws;
   const size_t T = s.tokens, H = s.hidden, I = s.intermediate, E = s.experts, R = r;
@@ -407,20 +411,21 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   w.scratch = align256((static_cast<size_t>(p->partitions) * E + blocks + 2 + E) * 4);
   w.source_rows = p->gather ? R * 4 : 0;
   if (is_int8(s)) {
-    w.x_q = T * int8_pitch(s.hidden);
-    w.x_scale = T * 4;
+    const size_t x_rows = p->gather ? T : R;   // one per token, or one per route in grouped order
+    w.x_q = x_rows * int8_pitch(s.hidden);
+    w.x_scale = x_rows * 4;
     w.activated_q = R * int8_pitch(s.intermediate);
     w.activated_scale = R * 4;
   }
   w.gathers = p->gather ? 1 : 0;
   w.down_tiles = p->down_tiles;
-  if (p->gather) w.grouped_input = 0;
+  if (p->gather || is_int8(s)) w.grouped_input = 0;
   w.token_tile = tile;
   w.schedule = schedule;
   w.launches = s.tokens == 0 ? 0 : (s.use_router ? 1 : 0) + (p->dispatch_fused ? 2 : 3) + (s.route_only ? 0 : 3);
   if (is_int8(s) && s.tokens) w.launches += 2;       // x and the activated rows are quantised
   if (s.route_only == 2) w.launches -= 1;            // no row copy
-  if (p->gather && p->dispatch_fused) w.launches -= 1;  // no row copy kernel
+  if ((p->gather || is_int8(s)) && p->dispatch_fused && s.tokens) w.launches -= 1;  // no row copy kernel
   if (s.external_dispatch) w.launches = s.tokens == 0 ? 0 : 2;  // gate_up + down only
   *out = p;
   return B200MOE_OK;
@@ -480,7 +485,7 @@ int b200moe_plan_bind(B200MoePlan* p, const B200MoeBuffers* b) {
     if (!s.external_dispatch)
       for (const Named& n : own_dispatch)
         if (!check(n)) return B200MOE_ERR_INVALID;
-    if (s.route_only != 2 && !p->gather && !check({b->grouped_input, "grouped_input"})) return B200MOE_ERR_INVALID;
+    if (s.route_only != 2 && !p->gather && !is_int8(s) && !check({b->grouped_input, "grouped_input"})) return B200MOE_ERR_INVALID;
     if (p->gather && !check({b->source_rows, "source_rows"})) return B200MOE_ERR_INVALID;
     if (is_int8(s)) {
       for (const Named& n : {Named{b->x_q, "x_q"}, Named{b->x_scale, "x_scale"}, Named{b->activated_q, "activated_q"},
@@ -607,7 +612,7 @@ int b200moe_dispatch(B200MoePlan* p, void* stream) {
 // Inside b200moe_forward the two BF16 tensor-core GEMMs are chained through per-expert counters.
 static bool w4_in_tmem(const B200MoePlan* p) { return p->token_tile <= 64; }
 static bool chain_stages(const B200MoePlan* p) {
-  if (is_int8(p->shape)) return false;
+  if (is_int8(p->shape)) return false;   // the rows are quantised in between
   if (p->shape.unchained || p->schedule != B200MOE_SCHEDULE_TCGEN05 || p->shape.external_dispatch == 1 || !p->buf.scratch)
     return false;
   const bool g4 = is_w4(p->shape.gate_up_format), d4 = is_w4(p->shape.down_format);

@@ -406,7 +406,7 @@ cudaError_t launch_dispatch(const B200MoePlan& p, cudaStream_t s) {
                                                     offsets, cursors, tasks, status, router_flag, valid, R, E,
                                                     p.warp_routes, p.token_tile, p.chain_words, source_rows, sh.topk);
     }
-    if (sh.route_only != 2 && !p.gather)  // the rows are sent to their expert owners / gathered by gate/up instead
+    if (sh.route_only != 2 && !p.gather && !p.int8)  // the rows are sent to their expert owners / gathered by gate/up instead
       launch_pdl(dispatch_copy_kernel, dim3((R + kWarps - 1) / kWarps), dim3(kThreads), 0, s,
           static_cast<const __nv_bfloat16*>(p.buf.x), static_cast<const int*>(mapping), static_cast<__nv_bfloat16*>(p.buf.grouped_input), R,
           sh.hidden, sh.topk);
@@ -424,7 +424,7 @@ cudaError_t launch_dispatch(const B200MoePlan& p, cudaStream_t s) {
       static_cast<int*>(p.buf.cursors), static_cast<int*>(p.buf.tasks), static_cast<int*>(p.buf.status),
       hist + router_flag_index(p), E, p.partitions, blocks, p.token_tile, p.chain_words);
   auto* x = static_cast<const __nv_bfloat16*>(p.buf.x);
-  auto* grouped = (sh.route_only == 2 || p.gather) ? nullptr : static_cast<__nv_bfloat16*>(p.buf.grouped_input);
+  auto* grouped = (sh.route_only == 2 || p.gather || p.int8) ? nullptr : static_cast<__nv_bfloat16*>(p.buf.grouped_input);
   int* source_rows = p.gather ? static_cast<int*>(p.buf.source_rows) : nullptr;
   if (grouped == nullptr) {
     const int mblocks = (R + kThreads - 1) / kThreads;

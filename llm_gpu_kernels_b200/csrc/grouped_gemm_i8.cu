@@ -10,7 +10,17 @@
 // gate/up: the two accumulators are the gate and the up rows of the same 128 channels; the epilogue scales both,
 // applies SwiGLU and stores FP32: the down product quantises these rows against their largest value, and rounding
 // them to BF16 first would move one in a hundred of the 8-bit values to its neighbour (0.8 % of the result).
-// product: the two accumulators are two neighbouring tiles of 128 channels (256 channels per tile share every row).
+// product: the two accumulators are two neighbouring tiles of 128 channels (256 channels per tile share every row), or
+// with one box per stage the even and the odd K steps of one tile of 128 channels, added in the epilogue.
+//
+// kSplit: few tiles for the SMs there are. A thread-block cluster works on one tile, each CTA on a slice of K; the
+// int32 partial sums meet through distributed shared memory (exact, so the split changes no bit either) and every CTA
+// finishes some of the rows.
+//
+// The kernel in front of this one (int8_quant.cu) lets its dependents start only after its own wait, so everything before
+// IT is complete and visible when this kernel starts: the dispatch's tables and the weights may be read at once, and
+// the first stages of weights are on their way while the rows are still being quantised. Only the rows, their scales
+// and the output wait.
 //
 // Bound by: HBM while a group has few rows (the weights are streamed once: 604 MB for 128 experts of 2048 x 768, half of
 // BF16), by operand bytes through L2 and shared memory beyond.
@@ -35,9 +45,10 @@ constexpr int kGatherThreads = kThreads + 32 * kGatherWarps;
 constexpr int kMaxStages = 12;
 constexpr int kRowBytes = 128;                       // K bytes of a stage
 constexpr uint32_t kBoxBytes = kTileM * kRowBytes;   // one weight box, 16 KB
-constexpr uint32_t kWBytes = 2 * kBoxBytes;
-constexpr int kCtrlBytes = 4096;
+constexpr int kCtrlBytes = 8192;
 constexpr int kMaxTile = 256;
+constexpr int kSplitSmem = kSmemLimit;
+constexpr int kMaxSplit = 8;
 
 struct Ctrl {
   uint64_t full[kMaxStages];
@@ -47,6 +58,7 @@ struct Ctrl {
   uint64_t drain[2];
   uint32_t tmem_base;
   int abort;
+  alignas(16) float row_scale[4][kMaxTile];   // of the tile an epilogue warp works on, a copy per warp
   Tables tables;
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block too large");
@@ -55,11 +67,30 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
 
-// kGateUp: SwiGLU epilogue (Out = float). kGather: token rows through source_rows.
-template <bool kGateUp, bool kGather, typename Out>
-__global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
+__device__ __forceinline__ float scaled(uint32_t sum, float scale) { return static_cast<float>(static_cast<int>(sum)) * scale; }
+__device__ __forceinline__ float swiglu(float gate, float up) { return (gate / (1.0f + __expf(-gate))) * up; }
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr, uint32_t cta) {
+  uint32_t remote;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote));
+  return v;
+}
+
+// kGateUp: SwiGLU epilogue (Out = float, two boxes). kGather: token rows through source_rows. kBoxes: weight boxes (tiles
+// of 128 channels) per stage. kSplit: one tile per cluster, K split over its CTAs.
+template <bool kGateUp, bool kGather, int kBoxes, bool kSplit, typename Out>
+__global__ void __launch_bounds__(kGather || kSplit ? kGatherThreads : kThreads, 1)
 grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
-  constexpr int kTileChannels = kGateUp ? kTileM : 2 * kTileM;
+  constexpr int kBlock = kGather || kSplit ? kGatherThreads : kThreads;   // a split product without gathering has four
+                                                                          // warps that only help with the partial sums
+  static_assert(!kGateUp || kBoxes == 2, "gate and up are the two boxes");
+  constexpr int kTileChannels = kGateUp ? kTileM : kBoxes * kTileM;
+  constexpr uint32_t kWBytes = kBoxes * kBoxBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Ctrl* c = reinterpret_cast<Ctrl*>(smem_raw);
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -88,8 +119,6 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc(&c->tmem_base, tmem_cols);
-  prefetch_head(g.prefetch_base, g.prefetch_chunks);   // HBM is idle while the kernels before this one run
-  pdl_wait();
   pdl_launch_dependents();
   if (g.tasks != nullptr) {
     load_tables(&c->tables, g.tasks, g.offsets, g.counts, E);
@@ -106,6 +135,20 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
   const int n_ct = (g.n_out + kTileChannels - 1) / kTileChannels;
   const int num_kb = (g.k + kRowBytes - 1) / kRowBytes;
   const int total_items = c->tables.tasks[E] * n_ct;
+  // the tiles of this CTA and the K blocks it does of them
+  int first_item = blockIdx.x, item_step = gridDim.x, kb0 = 0, kb1 = num_kb;
+  uint32_t cta = 0, ctas = 1;
+  if (kSplit) {   // one tile per cluster, a slice of its K blocks per CTA
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    const int per = (num_kb + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+    kb0 = min(num_kb, static_cast<int>(cta) * per);
+    kb1 = min(num_kb, kb0 + per);
+    first_item = kb0 < kb1 ? blockIdx.x / ctas : total_items;
+    item_step = total_items;
+  }
+  const bool any = first_item < total_items;
+  auto next_item = [&](int item) { return total_items - item > item_step ? item + item_step : total_items; };
 
   if (warp == 0) {
     if (lane == 0) {
@@ -116,16 +159,32 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       uint32_t phase = 0;
       long long issued = 0;
       bool ok = true;
-      for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
-        const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
+      auto load_weights = [&](const Tile& t, int kb, int st) {
+        unsigned char* to = stages + static_cast<size_t>(st) * stage_bytes;
         const int w_row = t.expert * g.w_rows + t.ct * kTileChannels;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&c->empty[stage], phase ^ 1u, &c->abort, g.status)) { ok = false; break; }
-          unsigned char* st = stages + static_cast<size_t>(stage) * stage_bytes;
-          mbar_expect_tx(&c->full[stage], kGather ? kWBytes : stage_bytes);
-          tma_load_2d(st, &g.tm_w, &c->full[stage], kb * kRowBytes, w_row, pol_w);
-          tma_load_2d(st + kBoxBytes, &g.tm_w, &c->full[stage], kb * kRowBytes, w_row + (kGateUp ? g.n_out : kTileM), pol_w);
-          if (!kGather) tma_load_2d(st + kWBytes, &g.tm_act, &c->full[stage], kb * kRowBytes, t.row0, pol_act);
+        mbar_expect_tx(&c->full[st], kGather ? kWBytes : stage_bytes);
+        tma_load_2d(to, &g.tm_w, &c->full[st], kb * kRowBytes, w_row, pol_w);
+        if (kBoxes == 2)
+          tma_load_2d(to + kBoxBytes, &g.tm_w, &c->full[st], kb * kRowBytes, w_row + (kGateUp ? g.n_out : kTileM), pol_w);
+      };
+      int early = 0;   // stages of the first tile whose weights are already on their way
+      if (any) {
+        const Tile t = decode_tile(&c->tables, first_item, E, n_ct, token_tile);
+        for (; early < num_stages && kb0 + early < kb1; ++early) load_weights(t, kb0 + early, early);
+      }
+      pdl_wait();
+      for (int item = first_item; ok && item < total_items; item = next_item(item)) {
+        const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (early > 0) {
+            --early;
+          } else {
+            if (!mbar_wait(&c->empty[stage], phase ^ 1u, &c->abort, g.status)) { ok = false; break; }
+            load_weights(t, kb, stage);
+          }
+          if (!kGather)
+            tma_load_2d(stages + static_cast<size_t>(stage) * stage_bytes + kWBytes, &g.tm_act, &c->full[stage],
+                        kb * kRowBytes, t.row0, pol_act);
           ++issued;
           if (++stage == num_stages) { stage = 0; phase ^= 1u; }
         }
@@ -147,22 +206,26 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
+      for (int item = first_item; ok && item < total_items; item = next_item(item)) {
         const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
         const uint32_t idesc = umma_idesc_i8(kTileM, t.n_eff);
         if (!mbar_wait(&c->tmem_empty[acc], acc_phase ^ 1u, &c->abort, g.status)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * acc_cols + half * token_tile);
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&c->full[stage], phase, &c->abort, g.status)) { ok = false; break; }
           tc_fence_after();
           if (kGather) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // cp.async-written rows -> MMA
           const uint32_t w_addr = smem_u32(stages + static_cast<size_t>(stage) * stage_bytes);
           const uint32_t a_addr = w_addr + kWBytes;
 #pragma unroll
-          for (int k = 0; k < kRowBytes / 32; ++k)
-            umma_i8(d, umma_desc(w_addr + half * kBoxBytes + k * 32), umma_desc(a_addr + k * 32), idesc,
-                    (kb | k) != 0 ? 1u : 0u);
+          for (int k = 0; k < kRowBytes / 32; ++k) {
+            if (kBoxes == 2)
+              umma_i8(d, umma_desc(w_addr + half * kBoxBytes + k * 32), umma_desc(a_addr + k * 32), idesc,
+                      kb != kb0 || k != 0 ? 1u : 0u);
+            else if ((k & 1) == half)
+              umma_i8(d, umma_desc(w_addr + k * 32), umma_desc(a_addr + k * 32), idesc, kb != kb0 || k > 1 ? 1u : 0u);
+          }
           umma_commit(&c->empty[stage]);
           if (++stage == num_stages) { stage = 0; phase ^= 1u; }
         }
@@ -181,10 +244,11 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
     const int gt = (warp - kMmaWarpB - 1) * 32 + lane;
     const int chunk = gt & 7;
     const int pitch = int8_pitch(g.k);
+    pdl_wait();
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
+    for (int item = first_item; ok && item < total_items; item = next_item(item)) {
       const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
       const int iters = (t.rows * 8 + 32 * kGatherWarps - 1) / (32 * kGatherWarps);
       int src[kIters];   // token of row it * 16 + gt / 8, -1 past the tile's rows
@@ -193,7 +257,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
         const int n = it * 16 + (gt >> 3);
         src[it] = (it < iters && n < t.rows) ? g.source_rows[t.row0 + n] : -1;
       }
-      for (int kb = 0; kb < num_kb; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         int free_ok = 1;
         if (lane == 0) free_ok = mbar_wait(&c->empty[stage], phase ^ 1u, &c->abort, g.status) ? 1 : 0;
         free_ok = __shfl_sync(0xffffffffu, free_ok, 0);
@@ -215,55 +279,132 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");   // never leave with copies in flight
-  } else {
+  } else if (warp < kMmaWarpB) {
     // ------------------------------------------------------------------ epilogue warps
     const int quarter = warp & 3;
-    Out* out = static_cast<Out*>(g.out);
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int item = blockIdx.x; item < total_items; item += gridDim.x) {
+    if (!kSplit) pdl_wait();   // row scales and output
+    for (int item = first_item; item < total_items; item = next_item(item)) {
       const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
-      const int channel = t.ct * kTileChannels + quarter * 32 + lane;      // of the first accumulator
+      const int channel = t.ct * kTileChannels + quarter * 32 + lane;      // of the first box
       const int channel_b = kGateUp ? channel : channel + kTileM;
-      const bool ok_a = channel < g.n_out, ok_b = channel_b < g.n_out;
+      const bool ok_a = channel < g.n_out, ok_b = kBoxes == 2 && channel_b < g.n_out;
       const float* scales = g.w_scale + static_cast<size_t>(t.expert) * g.w_rows;
-      const float sa = ok_a ? scales[channel] : 0.0f;
-      const float sb = ok_b ? scales[kGateUp ? g.n_out + channel : channel_b] : 0.0f;
+      const float sa = !kSplit && ok_a ? scales[channel] : 0.0f;
+      const float sb = !kSplit && ok_b ? scales[kGateUp ? g.n_out + channel : channel_b] : 0.0f;
+      // the tile's row scales while its MMAs still run: fetched chunk by chunk they cost two L2 round trips per 16 rows
+      float* row_scale = c->row_scale[quarter];
+      if (!kSplit)
+        for (int n = lane; n < t.n_eff; n += 32)
+          row_scale[n] = n < t.rows ? g.row_scale[kGather ? g.source_rows[t.row0 + n] : t.row0 + n] : 0.0f;
       if (!__all_sync(0xffffffffu, mbar_wait(&c->tmem_full[acc], acc_phase, &c->abort, g.status))) break;
+      __syncwarp();
       tc_fence_after();
       const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * acc_cols) + (static_cast<uint32_t>(quarter * 32) << 16);
-      Out* dst = out + static_cast<size_t>(t.row0) * g.n_out;
-      for (int n0 = 0; n0 < t.n_eff; n0 += 16) {
-        uint32_t a[16], b[16];
-        tmem_ld16(taddr + n0, a);
-        tmem_ld16(taddr + token_tile + n0, b);
-        // lane j holds the scale of row n0 + j
-        const int n_mine = n0 + (lane & 15);
-        float row_scale = 0.0f;
-        if (n_mine < t.rows) row_scale = g.row_scale[kGather ? g.source_rows[t.row0 + n_mine] : t.row0 + n_mine];
-        tmem_ld_wait();
+      if (kSplit) {
+        // partial sums [box][row][128], for the cluster, into the drained stages
+        int* part = reinterpret_cast<int*>(stages) + quarter * 32 + lane;
+        for (int n0 = 0; n0 < t.n_eff; n0 += 16) {
+          uint32_t a[16], b[16];
+          tmem_ld16(taddr + n0, a);
+          tmem_ld16(taddr + token_tile + n0, b);
+          tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int n = n0 + j;
-          const float s = __shfl_sync(0xffffffffu, row_scale, j);
-          const float va = static_cast<float>(static_cast<int>(a[j])) * (s * sa);
-          const float vb = static_cast<float>(static_cast<int>(b[j])) * (s * sb);
-          if (n < t.rows) {
-            Out* row = dst + static_cast<size_t>(n) * g.n_out;
-            if (kGateUp) {
-              if (ok_a) store_out(row + channel, (va / (1.0f + __expf(-va))) * vb);
-            } else {
-              if (ok_a) store_out(row + channel, va);
-              if (ok_b) store_out(row + channel_b, vb);
+          for (int j = 0; j < 16; ++j) {
+            part[(n0 + j) * kTileM] = static_cast<int>(kBoxes == 2 ? a[j] : a[j] + b[j]);
+            if (kBoxes == 2) part[(token_tile + n0 + j) * kTileM] = static_cast<int>(b[j]);
+          }
+        }
+      } else {
+        Out* dst = static_cast<Out*>(g.out) + static_cast<size_t>(t.row0) * g.n_out;
+        for (int n0 = 0; n0 < t.n_eff; n0 += 16) {
+          uint32_t a[16], b[16];
+          tmem_ld16(taddr + n0, a);
+          tmem_ld16(taddr + token_tile + n0, b);
+          float scale[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(scale + 4 * j) = *reinterpret_cast<const float4*>(row_scale + n0 + 4 * j);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int n = n0 + j;
+            const float s = scale[j];
+            if (n < t.rows) {
+              Out* row = dst + static_cast<size_t>(n) * g.n_out;
+              if constexpr (kGateUp) {
+                if (ok_a) store_out(row + channel, swiglu(scaled(a[j], s * sa), scaled(b[j], s * sb)));
+              } else if constexpr (kBoxes == 2) {
+                if (ok_a) store_out(row + channel, scaled(a[j], s * sa));
+                if (ok_b) store_out(row + channel_b, scaled(b[j], s * sb));
+              } else {
+                if (ok_a) store_out(row + channel, scaled(a[j] + b[j], s * sa));
+              }
             }
           }
         }
       }
       tc_fence_before();
-      __syncwarp();
+      __syncwarp();   // also: row_scale is read before the next tile's is written
       if (lane == 0) mbar_arrive(&c->tmem_empty[acc]);
       if (++acc == num_acc) { acc = 0; acc_phase ^= 1u; }
     }
+  }
+
+  if constexpr (kSplit) {
+    // ------------------------------------------------------------------ the cluster's partial sums -> output
+    __syncwarp();
+    cluster_barrier();   // every CTA's partial sums are in its shared memory
+    pdl_wait();          // row scales and output
+    const int tile = blockIdx.x / ctas;
+    if (tile < total_items && !*reinterpret_cast<volatile int*>(&c->abort)) {
+      const Tile t = decode_tile(&c->tables, tile, E, n_ct, token_tile);
+      const int per = (num_kb + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+      const int active = (num_kb + per - 1) / per;   // CTAs that had K blocks
+      const uint32_t base = smem_u32(stages) + static_cast<uint32_t>(lane) * 16u;
+      const float* scales = g.w_scale + static_cast<size_t>(t.expert) * g.w_rows;
+      Out* dst = static_cast<Out*>(g.out) + static_cast<size_t>(t.row0) * g.n_out;
+      // a unit is one row of one box (gate/up: of both); units go round the CTAs, then the warps
+      const int units = (kBoxes == 2 && !kGateUp ? 2 : 1) * t.rows;
+      for (int u = static_cast<int>(cta) + static_cast<int>(ctas) * warp; u < units;
+           u += static_cast<int>(ctas) * kBlock / 32) {
+        const int n = u % t.rows, box = u / t.rows;
+        const int channel = t.ct * kTileChannels + box * kTileM + lane * 4;
+        const float row_scale = g.row_scale[kGather ? g.source_rows[t.row0 + n] : t.row0 + n];
+        int sum[4] = {}, sum_up[4] = {};
+        int4 v[kMaxSplit], w[kGateUp ? kMaxSplit : 1];   // all loads first: one round trip
+#pragma unroll
+        for (int i = 0; i < kMaxSplit; ++i) {
+          if (i < active) {
+            v[i] = ld_cluster_int4(base + static_cast<uint32_t>((box * token_tile + n) * kTileM * 4), i);
+            if constexpr (kGateUp) w[i] = ld_cluster_int4(base + static_cast<uint32_t>((token_tile + n) * kTileM * 4), i);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kMaxSplit; ++i) {
+          if (i < active) {
+            sum[0] += v[i].x; sum[1] += v[i].y; sum[2] += v[i].z; sum[3] += v[i].w;
+            if constexpr (kGateUp) {
+              sum_up[0] += w[i].x; sum_up[1] += w[i].y; sum_up[2] += w[i].z; sum_up[3] += w[i].w;
+            }
+          }
+        }
+        Out* row = dst + static_cast<size_t>(n) * g.n_out + channel;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (channel + j < g.n_out) {
+            const float v = scaled(static_cast<uint32_t>(sum[j]), row_scale * scales[channel + j]);
+            if constexpr (kGateUp)
+              store_out(row + j, swiglu(v, scaled(static_cast<uint32_t>(sum_up[j]), row_scale * scales[g.n_out + channel + j])));
+            else
+              store_out(row + j, v);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_barrier();   // no CTA leaves while another may read its shared memory
   }
 
   tc_fence_before();
@@ -275,29 +416,60 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
   }
 }
 
-template <bool kGateUp, bool kGather, typename Out>
-cudaError_t launch(const I8Gemm& g, int grid, cudaStream_t s) {
+template <bool kGateUp, bool kGather, int kBoxes, bool kSplit, typename Out>
+cudaError_t launch(const I8Gemm& g, cudaStream_t s) {
   int smem = 0;
-  i8_stages(g.token_tile, &smem);
-  return launch_pdl(grouped_gemm_i8_kernel<kGateUp, kGather, Out>, dim3(grid), dim3(kGather ? kGatherThreads : kThreads),
-                    smem, s, g);
+  i8_stages(g.boxes, g.token_tile, g.split, &smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(g.grid);
+  cfg.blockDim = dim3(kGather || kSplit ? kGatherThreads : kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = g.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kSplit ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, grouped_gemm_i8_kernel<kGateUp, kGather, kBoxes, kSplit, Out>, g);
+}
+
+template <typename Out>
+cudaError_t launch_product(const I8Gemm& g, cudaStream_t s) {
+  if (g.split > 1) return g.boxes == 2 ? launch<false, false, 2, true, Out>(g, s) : launch<false, false, 1, true, Out>(g, s);
+  return g.boxes == 2 ? launch<false, false, 2, false, Out>(g, s) : launch<false, false, 1, false, Out>(g, s);
 }
 
 }  // namespace
 
-int i8_stages(int token_tile, int* smem_bytes) {
-  const int stage = static_cast<int>(kWBytes) + token_tile * kRowBytes;
-  int stages = (kSmemLimit - kCtrlBytes - 1024) / stage;
+int i8_stages(int boxes, int token_tile, int split, int* smem_bytes) {
+  const int stage = boxes * static_cast<int>(kBoxBytes) + token_tile * kRowBytes;
+  // the partial sums of a split tile take the place of the drained stages
+  const int partial = split > 1 ? boxes * token_tile * kTileM * 4 : 0;
+  const int space = (split > 1 ? kSplitSmem : kSmemLimit) - kCtrlBytes - 1024;
+  int stages = space / stage;
   if (stages > kMaxStages) stages = kMaxStages;
-  *smem_bytes = kCtrlBytes + 1024 + stages * stage;
+  *smem_bytes = kCtrlBytes + 1024 + (stages * stage > partial ? stages * stage : partial);
   return stages;
 }
 
 int configure_i8() {
-  const void* kernels[] = {reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, false, float>),
-                           reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, true, float>),
-                           reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, __nv_bfloat16>),
-                           reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, __half>)};
+  using bf16 = __nv_bfloat16;
+  const void* kernels[] = {
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, false, 2, false, float>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, true, 2, false, float>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, true, 2, true, float>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, false, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, true, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, false, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, true, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, false, __half>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, true, __half>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, false, __half>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, true, __half>)};
   for (const void* kernel : kernels) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (e != cudaSuccess) {
@@ -308,13 +480,13 @@ int configure_i8() {
   return B200MOE_OK;
 }
 
-cudaError_t launch_i8_gate_up(const I8Gemm& g, bool gather, int grid, cudaStream_t s) {
-  return gather ? launch<true, true, float>(g, grid, s) : launch<true, false, float>(g, grid, s);
+cudaError_t launch_i8_gate_up(const I8Gemm& g, cudaStream_t s) {
+  if (g.split > 1) return launch<true, true, 2, true, float>(g, s);
+  return g.source_rows != nullptr ? launch<true, true, 2, false, float>(g, s) : launch<true, false, 2, false, float>(g, s);
 }
 
-cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, int grid, cudaStream_t s) {
-  return out_dtype == B200MOE_FP16 ? launch<false, false, __half>(g, grid, s)
-                                   : launch<false, false, __nv_bfloat16>(g, grid, s);
+cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, cudaStream_t s) {
+  return out_dtype == B200MOE_FP16 ? launch_product<__half>(g, s) : launch_product<__nv_bfloat16>(g, s);
 }
 
 }  // namespace b200moe

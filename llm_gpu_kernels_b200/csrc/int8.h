@@ -18,6 +18,8 @@ struct QuantizeRows {
   int rows, k;
   int8_t* q;         // [rows, int8_pitch(k)]
   float* scale;      // [rows]
+  const int* mapping; // null, or [rows * copies]: the rows of q and scale that get row r (16-bit x)
+  int copies;
 };
 cudaError_t launch_quantize_rows(const QuantizeRows& a, cudaStream_t s);
 
@@ -45,16 +47,17 @@ struct I8Gemm {
   const int* counts;
   const int* tasks;
   int* status;
+  const int* source_rows;      // gathering: token of each row; else null
   const int8_t* x_q;           // gathering: [tokens, int8_pitch(k)]
-  const int* source_rows;      // gathering: token of each row
-  const unsigned char* prefetch_base;
-  int prefetch_chunks;
   int groups, rows, n_out, k, w_rows, token_tile, stages, stream_weights;
+  int boxes;                   // tiles of 128 channels per stage (gate/up: 2)
+  int split;                   // CTAs of a cluster that share a tile's K; 1: persistent CTAs, a tile each
+  int grid;
 };
-int i8_stages(int token_tile, int* smem_bytes);
+int i8_stages(int boxes, int token_tile, int split, int* smem_bytes);
 int configure_i8();   // opt-in shared memory of the kernels on the current device
-cudaError_t launch_i8_gate_up(const I8Gemm& g, bool gather, int grid, cudaStream_t s);
-cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, int grid, cudaStream_t s);
+cudaError_t launch_i8_gate_up(const I8Gemm& g, cudaStream_t s);   // gathers if source_rows is set
+cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, cudaStream_t s);
 // 2-D int8 tensor map, box 128 bytes x box_rows, 128-byte swizzle, zero fill past the ends.
 int encode_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows,
               bool weights);

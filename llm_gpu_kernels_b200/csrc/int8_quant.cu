@@ -13,13 +13,14 @@ using namespace rows8;
 constexpr int kThreads = 256;
 constexpr int kCached = 4;   // pieces of 8 values a thread keeps
 
-// L threads per row (a power of two, 32 .. 256).
-template <typename T, int L, bool kVec>
+// L threads per row (a power of two, 32 .. 256). kScatter: row r goes to the rows mapping[r * copies ..] of q and scale
+// instead of row r (the grouped rows of the token's routes; negative: none).
+template <typename T, int L, bool kVec, bool kScatter>
 __global__ void __launch_bounds__(kThreads)
 quantize_rows_kernel(const T* __restrict__ x, long long pitch, int8_t* __restrict__ q, float* __restrict__ scale,
-                     int rows, int K, int q_pitch) {
-  pdl_launch_dependents();
+                     int rows, int K, int q_pitch, const int* __restrict__ mapping, int copies) {
   pdl_wait();   // x may be written by the kernel before; q may still be read by it
+  pdl_launch_dependents();   // not earlier: a dependent relies on everything before this kernel being complete
   const int t = threadIdx.x & (L - 1);
   const int row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
   const bool live = row < rows;
@@ -47,17 +48,31 @@ quantize_rows_kernel(const T* __restrict__ x, long long pitch, int8_t* __restric
   }
   if (!live) return;
   const RowScale r = row_scale_of(bits);
-  if (t == 0) scale[row] = r.scale;
-  int8_t* dst = q + static_cast<size_t>(row) * q_pitch;
+  if (!kScatter && t == 0) scale[row] = r.scale;
+  if (kScatter)
+    for (int c = t; c < copies; c += L) {
+      const int to = mapping[static_cast<size_t>(row) * copies + c];
+      if (to >= 0) scale[to] = r.scale;
+    }
+  auto store = [&](int k, uint2 v8) {
+    if (!kScatter) {
+      *reinterpret_cast<uint2*>(q + static_cast<size_t>(row) * q_pitch + k) = v8;
+    } else {
+      for (int c = 0; c < copies; ++c) {
+        const int to = mapping[static_cast<size_t>(row) * copies + c];
+        if (to >= 0) *reinterpret_cast<uint2*>(q + static_cast<size_t>(to) * q_pitch + k) = v8;
+      }
+    }
+  };
 #pragma unroll
   for (int c = 0; c < kCached; ++c) {
     const int k = (c * L + t) * 8;
-    if (k < q_pitch) *reinterpret_cast<uint2*>(dst + k) = quantize8(v[c], r);
+    if (k < q_pitch) store(k, quantize8<sizeof(T) == 2>(v[c], r));
   }
   for (int k = (kCached * L + t) * 8; k < q_pitch; k += L * 8) {
     float u[8];
     load8<T, kVec>(src, k, K, u);
-    *reinterpret_cast<uint2*>(dst + k) = quantize8(u, r);
+    store(k, quantize8<sizeof(T) == 2>(u, r));
   }
 }
 
@@ -68,18 +83,21 @@ cudaError_t launch_rows(const QuantizeRows& a, cudaStream_t s) {
   const int per_block = kThreads / L;
   const dim3 grid((a.rows + per_block - 1) / per_block);
   const int q_pitch = int8_pitch(a.k);
-  return vec ? launch_pdl(quantize_rows_kernel<T, L, true>, grid, dim3(kThreads), 0, s, x, a.pitch, a.q, a.scale, a.rows,
-                          a.k, q_pitch)
-             : launch_pdl(quantize_rows_kernel<T, L, false>, grid, dim3(kThreads), 0, s, x, a.pitch, a.q, a.scale, a.rows,
-                          a.k, q_pitch);
+  auto go = [&](auto kernel) {
+    return launch_pdl(kernel, grid, dim3(kThreads), 0, s, x, a.pitch, a.q, a.scale, a.rows, a.k, q_pitch, a.mapping, a.copies);
+  };
+  if constexpr (sizeof(T) == 2)
+    if (a.mapping) return vec ? go(quantize_rows_kernel<T, L, true, true>) : go(quantize_rows_kernel<T, L, false, true>);
+  return vec ? go(quantize_rows_kernel<T, L, true, false>) : go(quantize_rows_kernel<T, L, false, false>);
 }
 
-// As few threads per row as keep the row in registers.
+// As few threads per row as keep the row in registers; with few rows, as many as have a piece to do (latency).
 template <typename T>
 cudaError_t launch_typed(const QuantizeRows& a, cudaStream_t s) {
-  if (a.k <= 32 * 8 * kCached) return launch_rows<T, 32>(a, s);
-  if (a.k <= 64 * 8 * kCached) return launch_rows<T, 64>(a, s);
-  if (a.k <= 128 * 8 * kCached) return launch_rows<T, 128>(a, s);
+  const int per = a.rows <= 256 ? 8 : 8 * kCached;
+  if (a.k <= 32 * per) return launch_rows<T, 32>(a, s);
+  if (a.k <= 64 * per) return launch_rows<T, 64>(a, s);
+  if (a.k <= 128 * per) return launch_rows<T, 128>(a, s);
   return launch_rows<T, 256>(a, s);
 }
 

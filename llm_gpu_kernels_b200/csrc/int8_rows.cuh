@@ -1,10 +1,7 @@
 // Rows to 8-bit integers, one scale per row:
 //   top = max |x_k|,  q_k = rint(127 x_k / top)  (ties to even),  scale = top / 127
 // A row of zeros gives zeros and scale 0; a row that holds an infinity or a NaN gives zeros and scale NaN, so every
-// product of it is NaN. q is that of exact arithmetic on the values read: x * (127 / top) in FP32 is off by at most
-// 2^-16 (two roundings of values up to 127), so only a quotient that close to a half may round the wrong way, and
-// those few are divided again in FP64 (where a 16-bit or 24-bit x over top cannot come closer to a half without being
-// one than 2^-33).
+// product of it is NaN. q is that of exact arithmetic on the values read (quantize8).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,24 +40,11 @@ __device__ __forceinline__ uint32_t top_bits(const float (&v)[8], uint32_t top) 
   return top;
 }
 
-// up: a power of two that lifts the row out of the subnormal range.
-__device__ __forceinline__ int round_to_int8(float x, float inverse, float top, float up) {
-  const float t = x * up * inverse, r = rintf(t);
-  if (fabsf(t - r) > 0.4999f) return static_cast<int>(rint(127.0 * static_cast<double>(x) * up / static_cast<double>(top)));
-  return static_cast<int>(r);
-}
-
-__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inverse, float top, float up) {
-  uint32_t w[2] = {0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    w[j >> 2] |= (static_cast<uint32_t>(round_to_int8(v[j], inverse, top, up)) & 0xffu) << (8 * (j & 3));
-  return make_uint2(w[0], w[1]);
-}
-
 // The factors of a row whose largest magnitude has the bits `bits`.
 struct RowScale {
-  float top, up, inverse, scale;
+  float up;                          // a power of two that keeps the row clear of overflow and of subnormals
+  float top, reciprocal, inverse;    // the largest magnitude times up, 1 / top, 127 / top
+  float scale;
   bool zero;   // all of q is 0: a row of zeros, or one that is not finite
 };
 __device__ __forceinline__ RowScale row_scale_of(uint32_t bits) {
@@ -68,14 +52,54 @@ __device__ __forceinline__ RowScale row_scale_of(uint32_t bits) {
   const bool finite = bits < 0x7f800000u;
   r.top = __uint_as_float(bits);
   r.scale = finite ? r.top / 127.0f : __uint_as_float(0x7fffffffu);
-  r.up = r.top < 1e-30f ? 0x1p100f : 1.0f;
+  r.up = r.top < 1e-30f ? 0x1p100f : r.top > 1e30f ? 0x1p-100f : 1.0f;
   r.top *= r.up;
   r.zero = !finite || bits == 0;
   r.inverse = r.zero ? 0.0f : 127.0f / r.top;
+  r.reciprocal = r.zero ? 0.0f : 1.0f / r.top;
   return r;
 }
+__device__ __forceinline__ uint2 pack8(const uint32_t (&b)[8]) {   // the low bytes
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
+// Eight values to eight bytes, six or seven instructions each. Adding 1.5 * 2^23 rounds to an integer, ties to even, and
+// leaves it in the low bits.
+// kHalf (16-bit values): 127 x is exact in FP32, and one correction with its exact remainder gives the quotient with an
+// error below 2^-16; a quotient that is a half exactly is representable and comes out exact, any other is at least
+// 2^-12 away from a half (denominators below 2^11): no quotient rounds the wrong way.
+// FP32 values: the quotient is off by up to 2^-16; where one of the eight is that close to a half, they are divided in FP64.
+template <bool kHalf>
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], const RowScale& r) {
-  return r.zero ? make_uint2(0u, 0u) : quantize8(v, r.inverse, r.top, r.up);
+  if (r.zero) return make_uint2(0u, 0u);
+  constexpr float kRound = 12582912.0f;
+  uint32_t b[8];
+  if (kHalf) {
+    const float factor = 127.0f * r.up;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float p = v[j] * factor;
+      const float t = p * r.reciprocal;
+      b[j] = __float_as_uint(__fadd_rn(fmaf(fmaf(-t, r.top, p), r.reciprocal, t), kRound));
+    }
+    return pack8(b);
+  }
+  float far = 0.0f;   // the largest distance from an integer
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = v[j] * r.inverse;
+    const float q = __fadd_rn(t, kRound);
+    far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(q, kRound))));
+    b[j] = __float_as_uint(q);
+  }
+  if (far > 0.49998f || r.up != 1.0f) {   // one test for all eight: a branch per value costs more than the rounding
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      b[j] = static_cast<uint32_t>(
+          static_cast<int>(rint(127.0 * static_cast<double>(v[j]) * r.up / static_cast<double>(r.top))));
+  }
+  return pack8(b);
 }
 
 }  // namespace rows8

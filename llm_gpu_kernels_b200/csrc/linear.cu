@@ -9,7 +9,7 @@ struct B200MoeLinear {
   B200MoeLinearBuffers buf{};
   bool bound = false;
   bool small = false;   // a few tokens: one kernel without tensor cores
-  int token_tile = 0, grid = 0, sms = 0;
+  int token_tile = 0, boxes = 2, split = 1, sms = 0;
   b200moe::I8Gemm gemm{};
 };
 
@@ -55,6 +55,8 @@ int b200moe_linear_create(const B200MoeLinearShape* shape, B200MoeLinear** out) 
   p->shape = *shape;
   p->small = linear_small_serves(shape->tokens, shape->k);
   p->token_tile = token_tile_of(shape->tokens);
+  if (shape->reserved[0]) p->token_tile = shape->reserved[0], p->boxes = shape->reserved[1], p->split = shape->reserved[2], p->small = false;
+  else if (shape->reserved[3]) p->small = shape->reserved[3] == 2;
   *out = p;
   return B200MOE_OK;
 }
@@ -134,11 +136,14 @@ int b200moe_linear_bind(B200MoeLinear* p, const B200MoeLinearBuffers* b) {
   g.k = s.k;
   g.w_rows = s.n;
   g.token_tile = p->token_tile;
+  g.boxes = p->boxes;
+  g.split = p->split;
   int smem = 0;
-  g.stages = i8_stages(p->token_tile, &smem);
+  g.stages = i8_stages(g.boxes, g.token_tile, g.split, &smem);
   g.stream_weights = s.tokens <= p->token_tile;
-  const long long items = static_cast<long long>((s.tokens + p->token_tile - 1) / p->token_tile) * ((s.n + 255) / 256);
-  p->grid = static_cast<int>(items < sms ? items : sms);
+  const long long items = static_cast<long long>((s.tokens + p->token_tile - 1) / p->token_tile) *
+                          ((s.n + 128 * p->boxes - 1) / (128 * p->boxes));
+  g.grid = static_cast<int>(p->split > 1 ? items * p->split : items < sms ? items : sms);
   p->bound = true;
   return B200MOE_OK;
 }
@@ -174,7 +179,7 @@ int b200moe_linear_forward(B200MoeLinear* p, void* cuda_stream) {
   q.q = static_cast<int8_t*>(p->buf.x_q);
   q.scale = static_cast<float*>(p->buf.x_scale);
   cudaError_t e = launch_quantize_rows(q, s);
-  if (e == cudaSuccess) e = launch_i8_product(p->gemm, p->shape.dtype, p->grid, s);
+  if (e == cudaSuccess) e = launch_i8_product(p->gemm, p->shape.dtype, s);
   if (e != cudaSuccess) {
     set_error("linear launch: %s", cudaGetErrorString(e));
     return B200MOE_ERR_CUDA;

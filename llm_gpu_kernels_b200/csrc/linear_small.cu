@@ -69,7 +69,7 @@ linear_small_kernel(const T* __restrict__ x, long long x_pitch, const int8_t* __
     for (int k = threadIdx.x * 8; k < smem_pitch; k += kThreads * 8) {
       float v[8] = {};
       if (r < tokens) load8<T, kVec>(x + r * x_pitch, k, K, v);
-      *reinterpret_cast<uint2*>(smem + r * smem_pitch + k) = quantize8(v, s);
+      *reinterpret_cast<uint2*>(smem + r * smem_pitch + k) = quantize8<true>(v, s);
     }
   }
   __syncthreads();

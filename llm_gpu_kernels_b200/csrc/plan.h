@@ -49,7 +49,8 @@ struct B200MoePlan {
   // the weight-streaming W4A16 kernel (token tile <= 16): dequantisation in registers, mma.sync
   int w4r_stages_gate_up = 0, w4r_smem_gate_up = 0;
   int w4r_stages_down = 0, w4r_smem_down = 0;
-  // INT8 plans: the two products
+  // INT8 plans: the two products; no BF16 rows are grouped
+  bool int8 = false;
   b200moe::I8Gemm i8_gate_up{}, i8_down{};
 };
 

@@ -313,7 +313,7 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
         plan = PreparedMoE(
             x, gate_up, down, ids, routing_weights, bf16((tokens, h)),
             int32((e,)), int32((e,)), int32((e,)), int32((e + 1,)), int32((r,)),
-            bf16((0 if sizes.gathers else r, h)), bf16((0, 2 * intermediate)),
+            bf16((0 if sizes.gathers or int8 else r, h)), bf16((0, 2 * intermediate)),
             torch.empty((0 if route_only_experts is not None else r, intermediate), device=device,
                         dtype=torch.float32 if int8 else torch.bfloat16), bf16((r, h)),
             int32((1,)), config,
@@ -325,8 +325,9 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             source_rows=int32((r,)) if sizes.gathers else None)
         if int8:
             byte = lambda rows, size: torch.empty((rows, size // max(1, rows)), device=device, dtype=torch.int8)
-            plan.x_q, plan.activated_q = byte(tokens, sizes.x_q), byte(r, sizes.activated_q)
-            plan.x_scale = torch.empty((tokens,), device=device, dtype=torch.float32)
+            x_rows = tokens if sizes.gathers else r
+            plan.x_q, plan.activated_q = byte(x_rows, sizes.x_q), byte(r, sizes.activated_q)
+            plan.x_scale = torch.empty((x_rows,), device=device, dtype=torch.float32)
             plan.activated_scale = torch.empty((r,), device=device, dtype=torch.float32)
         for name, tensor in (workspace or {}).items():  # caller-provided workspace (peer-visible buffers)
             if tuple(tensor.shape) != tuple(getattr(plan, name).shape) or tensor.dtype != getattr(plan, name).dtype:

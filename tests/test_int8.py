@@ -329,8 +329,14 @@ def check_layer(p, x, gate_up, down, ids, rw):
     t, k = ids.shape
     e, h, inter = down.shape
     q, scale = Q.quantize_rows(x)
-    assert torch.equal(base.x_q[:, :x.shape[1]].cpu().double(), q)
     counts, offsets, ranks, mapping = O.dispatch_oracle(ids, e)
+    x_q = base.x_q[:, :x.shape[1]].cpu().double()
+    assert base.gathers == (t * k <= 384 * e)
+    if base.gathers:      # one row per token
+        assert torch.equal(x_q, q)
+    else:                 # the routes' rows in grouped order
+        valid = mapping >= 0
+        assert torch.equal(x_q[mapping[valid].long()], q.repeat_interleave(k, 0)[valid])
     assert torch.equal(base.mapping.cpu(), mapping) and torch.equal(base.counts.cpu(), counts)
     values, scales = gate_up.values.cpu().double(), gate_up.scales.cpu().double()
     dvalues, dscales = down.values.cpu().double(), down.scales.cpu().double()
@@ -377,7 +383,7 @@ LAYER = [
     (17, 16, 4, 128, 96, "random", 0), (40, 8, 2, 256, 128, "random", 16), (40, 8, 2, 256, 128, "all_hot", 0),
     (33, 5, 3, 200, 130, "last_hot", 32), (64, 4, 2, 520, 264, "random", 64), (130, 4, 4, 128, 384, "random", 128),
     (300, 2, 1, 384, 256, "random", 256), (97, 32, 4, 1000, 72, "hot", 0), (50, 64, 8, 72, 40, "duplicate", 0),
-    (600, 6, 3, 136, 200, "random", 0), (5, 32, 4, 2048, 768, "random", 0), (1100, 3, 2, 256, 1100, "random", 0),
+    (600, 6, 3, 136, 200, "random", 0), (900, 2, 2, 131, 72, "random", 0), (500, 1, 1, 264, 256, "random", 0), (5, 32, 4, 2048, 768, "random", 0), (1100, 3, 2, 256, 1100, "random", 0),
 ]
 
 
