@@ -157,9 +157,6 @@ int bind_int8(B200MoePlan& p) {
   gu.stream_weights = static_cast<long long>(p.routes) <= static_cast<long long>(s.experts) * p.token_tile;
   gu.boxes = 2;
   gu.split = 1;
-  gu.grid = p.num_sms;
-  int smem = 0;
-  gu.stages = i8_stages(gu.boxes, p.token_tile, gu.split, &smem);
   dn = gu;
   gu.w_scale = static_cast<const float*>(b.gate_up_scales);
   gu.row_scale = static_cast<const float*>(b.x_scale);
@@ -175,6 +172,31 @@ int bind_int8(B200MoePlan& p) {
   dn.n_out = s.hidden;
   dn.k = s.intermediate;
   dn.w_rows = s.hidden;
+  // With few routes there are at most as many tiles per channel tile as routes: the form with the least estimated time.
+  // Otherwise pairs of channel tiles on persistent CTAs.
+  const long long row_tiles = (p.routes + p.token_tile - 1) / p.token_tile + s.experts - 1;
+  auto choose = [&](I8Gemm& g, int first_box) {
+    const long long most = row_tiles < p.routes ? row_tiles : p.routes;
+    const long long tiles = most * ((g.n_out + 127) / 128);
+    double best = -1.0;
+    if (tiles <= 2 * p.num_sms)
+      for (int boxes = first_box; boxes <= 2; ++boxes)
+        for (int split = 1; split <= (first_box == 1 || p.gather ? 8 : 1); split *= 2) {   // a split gate/up gathers
+          // gate/up has a channel tile of its own for each of its boxes' 128 channels
+          const double c = i8_cycles(most, first_box == 2 ? 2 * g.n_out : g.n_out, g.k, p.token_tile, boxes, split, p.num_sms);
+          if (c >= 0.0 && (best < 0.0 || c < best)) {
+            best = c;
+            g.boxes = boxes;
+            g.split = split;
+          }
+        }
+    int smem = 0;
+    g.stages = i8_stages(g.boxes, p.token_tile, g.split, &smem);
+    const long long items = most * ((g.n_out + (first_box == 2 ? 128 : 128 * g.boxes) - 1) / (first_box == 2 ? 128 : 128 * g.boxes));
+    g.grid = static_cast<int>(g.split > 1 ? items * g.split : items < p.num_sms ? items : p.num_sms);
+  };
+  choose(gu, 2);
+  choose(dn, 1);
   const uint64_t E = s.experts, I = s.intermediate, H = s.hidden;
   if ((rc = encode_i8(&gu.tm_w, b.gate_up, E * 2 * I, H, int8_pitch(s.hidden), 128, true))) return rc;
   if (!p.gather && (rc = encode_i8(&gu.tm_act, b.x_q, p.routes, H, int8_pitch(s.hidden), p.token_tile, false))) return rc;

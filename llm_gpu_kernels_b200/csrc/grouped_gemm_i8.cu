@@ -456,6 +456,31 @@ int i8_stages(int boxes, int token_tile, int split, int* smem_bytes) {
   return stages;
 }
 
+// What decides between tile shapes, with figures fitted to 33 timings of 9 to 2048 rows (k 1999 to 4096, n 1536 to 5003;
+// all but four within 12 %). A stage takes the longest of its bytes at 50 bytes per cycle out of L2, its MMAs (half a
+// cycle per row and K step of 32) and 210 cycles of hand-over; a tile that is not followed by another on its SM shows
+// its epilogue, 36 cycles per row and box; adding up a split tile takes 3200 cycles and 38 per row and box. Above 512
+// columns of accumulators there is only one set and every epilogue shows: 128 x 2 boxes in 25 rounds were faster than
+// 256 x 2 in 13 (393 and 451 us, 8192 x 4096 x 14336), so such tiles are for a single round only.
+double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxes, int split, int sms) {
+  const long long tiles = row_tiles * ((n_out + 128 * boxes - 1) / (128 * boxes));
+  const int blocks = (k + kRowBytes - 1) / kRowBytes;
+  int smem = 0;
+  if (i8_stages(boxes, token_tile, split, &smem) < 2 || smem > kSmemLimit) return -1.0;
+  const double bytes = boxes * static_cast<double>(kBoxBytes) + token_tile * kRowBytes;
+  double block = bytes / 50.0;
+  if (block < boxes * 2.0 * token_tile) block = boxes * 2.0 * token_tile;
+  if (block < 210.0) block = 210.0;
+  const double rows = static_cast<double>(token_tile) * boxes;
+  if (split > 1) {
+    if (tiles * split > sms || blocks < 2 * split) return -1.0;
+    return (blocks + split - 1) / split * block + 3200.0 + 38.0 * rows;
+  }
+  const double rounds = static_cast<double>((tiles + sms - 1) / sms);
+  if (rounds > 1 && 4 * token_tile > 512) return -1.0;
+  return rounds * blocks * block + 36.0 * rows;
+}
+
 int configure_i8() {
   using bf16 = __nv_bfloat16;
   const void* kernels[] = {

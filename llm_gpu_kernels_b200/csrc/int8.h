@@ -32,7 +32,7 @@ struct LinearSmall {
   void* y;
   int dtype, tokens, k, n, sms;
 };
-bool linear_small_serves(int tokens, int k);
+bool linear_small_serves(int tokens, int k, int n);
 cudaError_t launch_linear_small(const LinearSmall& a, cudaStream_t s);
 
 // One grouped product in int8 (grouped_gemm_i8.cu). Rows of group e are offsets[e] .. + counts[e] of the activations, or
@@ -55,6 +55,9 @@ struct I8Gemm {
   int grid;
 };
 int i8_stages(int boxes, int token_tile, int split, int* smem_bytes);
+// Cycles that a product of `row_tiles` tiles of `token_tile` rows with n_out channels and k values would take in the
+// given form, or -1 where the form does not exist. See grouped_gemm_i8.cu.
+double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxes, int split, int sms);
 int configure_i8();   // opt-in shared memory of the kernels on the current device
 cudaError_t launch_i8_gate_up(const I8Gemm& g, cudaStream_t s);   // gathers if source_rows is set
 cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, cudaStream_t s);

@@ -9,17 +9,30 @@ struct B200MoeLinear {
   B200MoeLinearBuffers buf{};
   bool bound = false;
   bool small = false;   // a few tokens: one kernel without tensor cores
-  int token_tile = 0, boxes = 2, split = 1, sms = 0;
+  int token_tile = 16, boxes = 1, split = 1, sms = 0;
   b200moe::I8Gemm gemm{};
 };
 
 namespace b200moe {
 namespace {
 
-int token_tile_of(int tokens) {
-  int tile = 16;
-  while (tile < 128 && tile < tokens) tile <<= 1;
-  return tile;
+constexpr int kSms = 148;   // B200; the schedule is chosen before a device is touched
+
+// Tile rows, boxes and K split with the least estimated time.
+void choose_tiles(B200MoeLinear* p) {
+  const B200MoeLinearShape& s = p->shape;
+  double best = -1.0;
+  for (int boxes = 1; boxes <= 2; ++boxes)
+    for (int tile = 16; tile <= 256 && (tile == 16 || tile - 16 < s.tokens); tile += 16)
+      for (int split = 1; split <= 8; split *= 2) {
+        const double c = i8_cycles((s.tokens + tile - 1) / tile, s.n, s.k, tile, boxes, split, kSms);
+        if (c >= 0.0 && (best < 0.0 || c < best)) {
+          best = c;
+          p->token_tile = tile;
+          p->boxes = boxes;
+          p->split = split;
+        }
+      }
 }
 
 }  // namespace
@@ -53,10 +66,8 @@ int b200moe_linear_create(const B200MoeLinearShape* shape, B200MoeLinear** out) 
     return B200MOE_ERR_INVALID;
   }
   p->shape = *shape;
-  p->small = linear_small_serves(shape->tokens, shape->k);
-  p->token_tile = token_tile_of(shape->tokens);
-  if (shape->reserved[0]) p->token_tile = shape->reserved[0], p->boxes = shape->reserved[1], p->split = shape->reserved[2], p->small = false;
-  else if (shape->reserved[3]) p->small = shape->reserved[3] == 2;
+  p->small = linear_small_serves(shape->tokens, shape->k, shape->n);
+  choose_tiles(p);
   *out = p;
   return B200MOE_OK;
 }

@@ -1,9 +1,9 @@
-// The dense 8-bit product for a few tokens (a decode step): one launch, no tensor cores.
+// The dense 8-bit product for one or two tokens (a decode step): one launch, no tensor cores.
 // Every block quantises the rows of x into its shared memory (int8_rows.cuh; a few KB out of L2, hidden behind the first
 // weight loads, which are issued before), then its warps take output channels in turn: 32 lanes read 512 bytes of a
 // weight row at a time, 16 bytes each, multiply with four-way integer dot products and add up with one warp reduction.
-// Bound by the stream of weights (N * K bytes, read once whatever the number of tokens) and for a small weight by
-// launch and load latency; two launches through the tensor-core kernel took 11.6 us for 1 x 2048 x 1536.
+// Bound by the stream of weights (N * K bytes, read once) and for a small weight by
+// launch and load latency: 3.0 us for 1 x 2048 x 1536, 6.4 us for 4096 x 4096, 12.4 us for 4096 x 14336 (4.75 TB/s).
 #include "int8.h"
 #include "int8_rows.cuh"
 #include "pdl.cuh"
@@ -129,17 +129,18 @@ cudaError_t launch(const LinearSmall& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t launch_typed(const LinearSmall& a, cudaStream_t s) {
-  if (a.tokens == 1) return launch<T, 1, 1>(a, s);
-  if (a.tokens == 2) return launch<T, 2, 2>(a, s);
-  return a.tokens <= 4 ? launch<T, 4, 2>(a, s) : launch<T, 8, 2>(a, s);
+  return a.tokens == 1 ? launch<T, 1, 1>(a, s) : launch<T, 2, 2>(a, s);
 }
 
 }  // namespace
 
-// At most eight tokens, and their quantised rows within the shared memory a block has without opting in.
-bool linear_small_serves(int tokens, int k) {
-  const int rows = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
-  return tokens <= 8 && static_cast<long long>(rows) * smem_pitch_of(k) <= 46 * 1024;
+// One token, or two with a weight of at most 32 MB: the second token costs as much again in dot products and shared
+// memory reads, the tensor cores nothing (two tokens: 4.4 against 6.2 us at 2048 x 1536, 8.3 against 9.6 at 4096 x 4096,
+// 19.5 against 15.8 at 4096 x 14336; four tokens would take 7.1, 12.5 and 27 us). Their quantised rows have to fit the
+// shared memory a block has without opting in.
+bool linear_small_serves(int tokens, int k, int n) {
+  return (tokens == 1 || (tokens == 2 && static_cast<long long>(n) * k <= 32ll << 20)) &&
+         static_cast<long long>(tokens) * smem_pitch_of(k) <= 46 * 1024;
 }
 
 cudaError_t launch_linear_small(const LinearSmall& a, cudaStream_t s) {

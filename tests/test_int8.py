@@ -383,7 +383,8 @@ LAYER = [
     (17, 16, 4, 128, 96, "random", 0), (40, 8, 2, 256, 128, "random", 16), (40, 8, 2, 256, 128, "all_hot", 0),
     (33, 5, 3, 200, 130, "last_hot", 32), (64, 4, 2, 520, 264, "random", 64), (130, 4, 4, 128, 384, "random", 128),
     (300, 2, 1, 384, 256, "random", 256), (97, 32, 4, 1000, 72, "hot", 0), (50, 64, 8, 72, 40, "duplicate", 0),
-    (600, 6, 3, 136, 200, "random", 0), (900, 2, 2, 131, 72, "random", 0), (500, 1, 1, 264, 256, "random", 0), (5, 32, 4, 2048, 768, "random", 0), (1100, 3, 2, 256, 1100, "random", 0),
+    (600, 6, 3, 136, 200, "random", 0), (900, 2, 2, 131, 72, "random", 0), (500, 1, 1, 264, 256, "random", 0), (500, 1, 1, 2048, 64, "random", 0),
+    (400, 1, 1, 4100, 40, "random", 16), (1, 1, 1, 5000, 700, "random", 0), (5, 32, 4, 2048, 768, "random", 0), (1100, 3, 2, 256, 1100, "random", 0),
 ]
 
 
