@@ -14,17 +14,16 @@
 // Precision: the weights are FP32. The CHOICE is that of exact arithmetic: where c comes from exp() in FP32, two
 // values closer than the error bound of that computation could be in the wrong order, so a row in which two
 // neighbours of the order (or the groups at the border) are that close is routed again in FP64 (route_exact): one row
-// in a few hundred for random logits.
+// in a thousand for random logits.
 //
 // What bounds the common pass (route_fast) at many rows is the number of instructions per row, so it keeps the experts
-// of a lane as sorted 32-bit keys: the order-preserving bits of c, of which the lowest three are replaced by the place
-// in the lane. Sorting eight is 19 compare-exchanges of two integer min / max; each of the K rounds is one maximum
-// over the lanes, one ballot and a shift of the winner's list. The K weights are computed at the end by K lanes at
-// once, from logits read again, so full-precision exp and division cost one instruction sequence per row.
-// 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups: 80 us with unsorted keys and per-expert weights (1930 warp
-// instructions per row), 47 us like this (910 instructions; 5.4 us would be the HBM floor). Sixteen experts per lane and
-// two rows per warp need as many instructions per row (935: the warp-wide redux of 32 lanes becomes four shuffles) and
-// more registers: 73 us.
+// of a lane as sorted 32-bit keys that hold the expert too: sorting eight is 19 compare-exchanges of two integer min /
+// max, each of the K rounds one maximum over the lanes and a shift of the winner's list. The K weights are computed at
+// the end by K lanes at once, from logits read again, so full-precision exp and division cost one instruction sequence
+// per row. 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups (5.4 us would be the HBM floor): 80 us with unsorted
+// keys and per-expert weights (1930 warp instructions per row), 47 us with sorted keys that leave ties and experts to
+// ballots (910), 41 us like this (895 instructions for a row that FP32 settles: 33 us if all did). Sixteen experts per lane and two rows per warp need as many instructions per row (the
+// warp-wide redux of 32 lanes becomes four shuffles) and more registers: 73 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -45,11 +44,6 @@ struct Config {
 };
 
 constexpr int kMaxGroups = 32;
-// |c_fp32 - c| <= kScoreError * (s_max + |c|) as route_fast computes c: __expf within 2^-22 + |l| 2^-23 relative
-// (weighted by the score: |d| exp(d) <= 0.37), up to 13 additions of a softmax sum (8 in a lane, 5 levels of the tree),
-// an approximate division and the bias addition stay below 1.5e-6; the three dropped key bits are 7 ulp, 8.4e-7 of |c|.
-constexpr float kScoreError = 2.5e-6f;
-
 template <typename F> struct Key;
 template <> struct Key<float> {
   using type = uint32_t;
@@ -120,8 +114,22 @@ __device__ __forceinline__ double score_of(const Config& cfg, double x, double t
 }
 
 // ------------------------------------------------------------------------------------------------ FP64, any row
-// load(e): the logit of expert e; wanted: this row is to be written (the other rows of the warp only take part). Not inlined: the rare pass must not cost the common one registers; it keeps one
-// 64-bit key per expert and computes the rest when needed.
+// The largest 64-bit key of a row. For a whole warp two integer reductions, of the high and of the low words, are less
+// than half as long as five steps of 64-bit shuffles.
+template <int L>
+__device__ __forceinline__ unsigned long long sub_max64(unsigned long long v) {
+  if constexpr (L == 32) {
+    const uint32_t hi = static_cast<uint32_t>(v >> 32), top = __reduce_max_sync(kAll, hi);
+    const uint32_t low = __reduce_max_sync(kAll, hi == top ? static_cast<uint32_t>(v) : 0u);
+    return static_cast<unsigned long long>(top) << 32 | low;
+  } else {
+    return sub_max<L>(v);
+  }
+}
+
+// load(e): the logit of expert e; wanted: this row is to be written (the other rows of the warp only take part). Not
+// inlined: the rare pass must not cost the common one registers. One warp in it holds up its SM's last rows, so it is
+// kept short as well: sorted keys as in route_fast, whole-warp reductions.
 template <int P, int L, typename Load>
 __device__ __noinline__ void route_exact(const Config& cfg, const float* __restrict__ bias, int lane, bool wanted,
                                          const Load& load, const Out& out) {
@@ -129,25 +137,27 @@ __device__ __noinline__ void route_exact(const Config& cfg, const float* __restr
   using KeyT = K::type;
   const double none = -INFINITY;
   auto logit = [&](int e) { return e < cfg.E ? fmaxf(load(e), -INFINITY) : -INFINITY; };   // NaN -> -inf
-  double top = none, sum = 0.0;
+  double v[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) v[j] = logit(lane * P + j);
+  double top = none, sum = 1.0;
   if (!cfg.sigmoid) {
-#pragma unroll 1
-    for (int j = 0; j < P; ++j) top = max(top, static_cast<double>(logit(lane * P + j)));
-    top = sub_max<L>(top);
-#pragma unroll 1
-    for (int j = 0; j < P; ++j) sum += score_of(cfg, logit(lane * P + j), top, 1.0);
+#pragma unroll
+    for (int j = 0; j < P; ++j) top = max(top, v[j]);
+    top = K::value(sub_max64<L>(K::of(top)));
+    sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) sum += score_of(cfg, v[j], top, 1.0);
     sum = sub_sum<L>(sum);
   }
-  KeyT key[P];   // 0: not a candidate
+  KeyT key[P];   // sorted, 0: not a candidate
+  int place[P];  // of key[j] in the lane
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    const int e = lane * P + j;
-    const double x = logit(e);
-    key[j] = 0;
-    if (x > none) {
-      const double b = bias != nullptr ? bias[e] : 0.0;
-      if (b > none) key[j] = K::of(bias != nullptr ? score_of(cfg, x, top, sum) + b : x);   // false for NaN
-    }
+    const float b = bias != nullptr && lane * P + j < cfg.E ? bias[lane * P + j] : 0.0f;
+    const double c = bias != nullptr ? score_of(cfg, v[j], top, sum) + static_cast<double>(b) : v[j];
+    key[j] = v[j] > none && b > -INFINITY ? K::of(c) : 0ull;   // false for NaN
+    place[j] = j;
   }
   if (cfg.kept < cfg.groups) {
     const int size = cfg.size;
@@ -161,19 +171,16 @@ __device__ __noinline__ void route_exact(const Config& cfg, const float* __restr
         b = max(b, min(a, x));
         a = max(a, x);
       }
-#pragma unroll
-      for (int o = 1; o < L; o <<= 1) {
-        const KeyT oa = __shfl_xor_sync(kAll, a, o), ob = __shfl_xor_sync(kAll, b, o);
-        b = max(min(a, oa), max(b, ob));
-        a = max(a, oa);
-      }
+      const KeyT first = sub_max64<L>(a);
+      const unsigned holder = sub_ballot<L>(a == first);   // its lowest lane gives up its largest
+      const KeyT second = sub_max64<L>(lane == lowest_lane(holder) ? b : a);
       double value = none;
-      if (a) {
-        value = K::value(a);
+      if (first) {
+        value = K::value(first);
         if (cfg.group_top2) {
           const bool scores = bias == nullptr;   // c is the score then, the keys are logits
           if (scores) value = score_of(cfg, value, top, sum);
-          if (b) value += scores ? score_of(cfg, K::value(b), top, sum) : K::value(b);
+          if (second) value += scores ? score_of(cfg, K::value(second), top, sum) : K::value(second);
         }
       }
 #pragma unroll
@@ -191,40 +198,51 @@ __device__ __noinline__ void route_exact(const Config& cfg, const float* __restr
 #pragma unroll
       for (int i = 0; i < kMaxGroups / L; ++i) {
         const int other = lane + i * L;
-        if (other < cfg.groups) before += mine[i] > value || (mine[i] == value && other < g) ? 1 : 0;
+        before += __popc(sub_ballot<L>(other < cfg.groups && (mine[i] > value || (mine[i] == value && other < g))));
       }
-      before = sub_sum<L>(before);
       kept_groups |= before < cfg.kept ? 1u << g : 0u;
     }
 #pragma unroll
     for (int j = 0; j < P; ++j)
       if (key[j] && !(kept_groups >> ((lane * P + j) / size) & 1u)) key[j] = 0;
   }
+  // descending, equal keys in the order of their places
+#pragma unroll
+  for (int r = 0; r < P; ++r)
+#pragma unroll
+    for (int i = r & 1; i + 1 < P; i += 2) {
+      if (key[i] < key[i + 1]) {
+        const KeyT k = key[i];
+        key[i] = key[i + 1];
+        key[i + 1] = k;
+        const int q = place[i];
+        place[i] = place[i + 1];
+        place[i + 1] = q;
+      }
+    }
   int expert = 0;                         // lane k: the expert of slot k
   bool filled = false;
   unsigned chosen = 0;                    // of this lane's experts
   for (int k = 0; k < cfg.K; ++k) {
-    KeyT best = key[0];
-#pragma unroll
-    for (int j = 1; j < P; ++j) best = max(best, key[j]);
-    const KeyT winner = sub_max<L>(best);
+    const KeyT winner = sub_max64<L>(key[0]);
     const bool empty = winner == 0;       // nobody left: the lowest index not chosen yet, with weight 0
-    int place = 0;                        // of the winner among this lane's experts, if it is here
-#pragma unroll
-    for (int j = P - 1; j >= 0; --j)
-      if (empty ? !(chosen >> j & 1u) : key[j] == winner) place = j;
-    const bool holds = empty ? chosen != (1u << P) - 1u && lane * P + place < cfg.E : best == winner;
+    int mine = place[0];
+    if (empty) mine = __ffs(static_cast<int>(~chosen)) - 1;
+    const bool holds = empty ? mine < P && lane * P + mine < cfg.E : key[0] == winner;
     const int owner = lowest_lane(sub_ballot<L>(holds));   // the lowest lane holds the lowest index
-    place = __shfl_sync(kAll, place, owner, L);
+    const int at = __shfl_sync(kAll, mine, owner, L);
     if (lane == k) {
-      expert = owner * P + place;
+      expert = owner * P + at;
       filled = !empty;
     }
     if (lane == owner) {
-      chosen |= 1u << place;
+      chosen |= 1u << at;
 #pragma unroll
-      for (int j = 0; j < P; ++j)
-        if (j == place) key[j] = 0;
+      for (int j = 0; j + 1 < P; ++j) {
+        key[j] = key[j + 1];
+        place[j] = place[j + 1];
+      }
+      key[P - 1] = 0;
     }
   }
   double w = lane < cfg.K && filled ? score_of(cfg, logit(expert), top, sum) : 0.0;
@@ -256,76 +274,111 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[P]) {
           if (i + j + d < P && (i + j) / (2 * p) == (i + j + d) / (2 * p)) exchange(k[i + j], k[i + j + d]);
 }
 
-constexpr uint32_t kPlaceBits = 7u;          // P <= 8
-constexpr uint32_t kNoneKey = 0x007fffffu;   // Key<float>::of(-INFINITY); every candidate's key is larger
-
 // Returns false when FP32 cannot settle the row; otherwise slot `lane` < K of the row is `expert` with weight `w`.
 // l[j]: logits of experts lane*P + j, b[j]: biases.
+//
+// Keys are (q << 8) | (255 - expert): the larger key has the larger q, or the lower index at equal q, so every key is
+// different, the winner of a round names its expert and no tie needs a second look. q has 24 bits and is at least 1
+// (key 0: not a candidate). Logits of 16 bits without a bias give their leading 24 bits, which are exact. Everything
+// else gives its place between the smallest and the largest c of the row (values below -1e30 count as the smallest):
+// q = 1 + (c - base) * scale, monotonic in c and off by less than 2 from rounding.
 template <int P, int L, typename Load>
 __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], const float (&b)[P], bool biased, int lane,
                                            const Load& load, int* expert, float* weight) {
   using K = Key<float>;
   const float none = -INFINITY;
   const bool grouped = cfg.kept < cfg.groups;
-  uint32_t key[P];
-  uint32_t low_bits = 0;
   float top = none;
+  uint32_t low_bits = 0;
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     l[j] = fmaxf(l[j], none);   // NaN -> -inf
     low_bits |= __float_as_uint(l[j]);
     top = fmaxf(top, l[j]);
   }
-  float unit = 1.0f, sum = 1.0f, widest = 0.0f;   // unit: the largest score there can be
-  if (!cfg.sigmoid) {
-    const uint32_t t = sub_max<L>(K::of(top));
-    top = K::value(t);
-    if (biased || grouped || !cfg.renormalize) {
-      sum = 0.0f;
+  top = K::value(sub_max<L>(K::of(top)));
+  float unit = 1.0f, sum = 1.0f;   // unit: the largest score there can be
+  if (!cfg.sigmoid && (biased || grouped || !cfg.renormalize)) {
+    sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < P; ++j) sum += l[j] > none ? __expf(l[j] == top ? 0.0f : l[j] - top) : 0.0f;
-      sum = sub_sum<L>(sum);
-      unit = __fdividef(1.0f, sum);
-    }
+    for (int j = 0; j < P; ++j) sum += l[j] > none ? __expf(l[j] == top ? 0.0f : l[j] - top) : 0.0f;
+    sum = sub_sum<L>(sum);
+    unit = __fdividef(1.0f, sum);
   }
   auto score = [&](float x) {   // approximate; for the choice only
     return cfg.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x)) : unit * __expf(x == top ? 0.0f : x - top);
   };
+  // Without a bias c is the logit; 16-bit logits, even as FP32, have nothing in their last 8 bits. One answer for the
+  // warp: the rows it routes are of one tensor.
+  const bool exact = !biased && __all_sync(kAll, (low_bits & 255u) == 0);
+  float c[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) c[j] = l[j];
   if (biased) {
     if (cfg.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < P; ++j)
-        key[j] = K::of(fmaxf(l[j] > none ? __fdividef(1.0f, 1.0f + __expf(-l[j])) + b[j] : none, none));
+      for (int j = 0; j < P; ++j) c[j] = fmaxf(l[j] > none ? __fdividef(1.0f, 1.0f + __expf(-l[j])) + b[j] : none, none);
     } else {
 #pragma unroll
-      for (int j = 0; j < P; ++j)
-        key[j] = K::of(fmaxf(l[j] > none ? unit * __expf(l[j] == top ? 0.0f : l[j] - top) + b[j] : none, none));
+      for (int j = 0; j < P; ++j) c[j] = fmaxf(l[j] > none ? unit * __expf(l[j] == top ? 0.0f : l[j] - top) + b[j] : none, none);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < P; ++j) key[j] = K::of(l[j]);
   }
-  // without a bias c is the logit itself: nothing is lost if its last bits are zero anyway (16-bit logits, even as FP32)
-  const bool exact = !biased && sub_ballot<L>((low_bits & kPlaceBits) != 0) == 0;
-#pragma unroll
-  for (int j = 0; j < P; ++j) key[j] = (key[j] & ~kPlaceBits) | (kPlaceBits - j);
-  sort_keys<P>(key);
+  uint32_t key[P];
+  float base = 0.0f, step = 0.0f;    // c = base + (q - 1) * step, about
+  uint32_t unsure = 0;               // two q this close or closer may be in the wrong order
   bool close = false;
+  if (exact) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) key[j] = c[j] > none ? (K::of(c[j]) & ~255u) | (255u - (lane * P + j)) : 0u;
+  } else {
+    float low = INFINITY, high = none;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      low = fminf(low, c[j] > -1e30f ? c[j] : INFINITY);
+      high = fmaxf(high, c[j]);
+    }
+    if (biased) high = K::value(sub_max<L>(K::of(high)));
+    else high = top;
+    low = -K::value(sub_max<L>(K::of(-low)));
+    low = fminf(low, high);
+    const float range = high - low;
+    // a row of one value, or with an infinity: every q is the same, which settles nothing
+    const float scale = range > 1e-30f && range < INFINITY ? 16777212.0f / range : 0.0f;
+    base = low;
+    step = scale > 0.0f ? range / 16777212.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const float q = fmaxf(0.0f, (c[j] - low) * scale) + 1.0f;   // NaN (infinities) -> 1
+      key[j] = c[j] > none ? __float2uint_rn(q) << 8 | (255u - (lane * P + j)) : 0u;
+    }
+    // The error of c: __expf is within 2^-22 + |x| 2^-23, which moves a sigmoid by a quarter of that and a softmax score
+    // by its own size times it (|x| exp(x) <= 0.37); a reciprocal of 2^-23; up to 13 additions of a softmax sum (8 in a
+    // lane, 5 levels of the tree): 4e-7 for a sigmoid, 1.5e-6 of the largest score for a softmax, and half an ulp of c.
+    if (biased) {
+      const float widest = fmaxf(fabsf(low), fabsf(high));
+      unsure = static_cast<uint32_t>(fminf(2.0f * ((cfg.sigmoid ? 4e-7f : 1.5e-6f * unit) + 6e-8f * widest) * scale + 5.0f, 16777215.0f));
+    }
+  }
+  sort_keys<P>(key);
   if (grouped) {
     const int lanes = cfg.size / P;   // a whole power of two: see route_row
-    float a = K::value(key[0] & ~kPlaceBits), second = P > 1 ? K::value(key[P > 1] & ~kPlaceBits) : none;
-    a = key[0] > kNoneKey ? a : none;
-    second = P > 1 && key[P > 1] > kNoneKey ? second : none;
+    uint32_t a = key[0], second = P > 1 ? key[P > 1] : 0u;
     for (int o = 1; o < lanes; o <<= 1) {
-      const float oa = __shfl_xor_sync(kAll, a, o), ob = __shfl_xor_sync(kAll, second, o);
-      second = fmaxf(fminf(a, oa), fmaxf(second, ob));
-      a = fmaxf(a, oa);
+      const uint32_t oa = __shfl_xor_sync(kAll, a, o), ob = __shfl_xor_sync(kAll, second, o);
+      second = max(min(a, oa), max(second, ob));
+      a = max(a, oa);
     }
+    auto value_of = [&](uint32_t k) {
+      return exact ? K::value(k & ~255u) : base + static_cast<float>((k >> 8) - 1u) * step;
+    };
     const bool by_score = cfg.group_top2 && !biased;
-    float value = a;
-    if (cfg.group_top2 && a != none) {
-      if (by_score) value = score(a);
-      if (second != none) value += by_score ? score(second) : second;
+    float value = none;
+    if (a) {
+      value = value_of(a);
+      if (cfg.group_top2) {
+        if (by_score) value = score(value);
+        if (second) value += by_score ? score(value_of(second)) : value_of(second);
+      }
     }
     const int leader = lane & ~(lanes - 1);   // of this lane's group
     uint32_t group_key = lane == leader && lane * P < cfg.E ? K::of(value) : 0u;
@@ -337,16 +390,11 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       kept |= leader == winner;
       if (lane == winner) group_key = 0u;
     }
-    if (__any_sync(kAll, !exact) || by_score) {   // is the border between the kept groups and the others certain?
-      const uint32_t next = sub_max<L>(group_key);
-      if (biased || by_score) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) widest = fmaxf(widest, fabsf(b[j]));
-        widest = __uint_as_float(sub_max<L>(__float_as_uint(widest)));
-        close = K::value(last) - K::value(next) <= 4.0f * kScoreError * (unit + widest);   // infinities compare false
-      } else {
-        close = !exact && last == next && last != kNoneKey;
-      }
+    if (!exact || by_score) {   // is the border between the kept groups and the others certain?
+      const float border = K::value(last), next = K::value(sub_max<L>(group_key));
+      // two values of two c each (or scores, whose logits are off by `step`)
+      const float far = by_score ? 4.0f * (2e-6f * unit + step) : 2.0f * step * static_cast<float>(unsure + 2u) + 2.4e-7f * fabsf(border);
+      close = border - next <= far;   // infinities compare false
     }
     if (!kept) {
 #pragma unroll
@@ -354,41 +402,25 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
     }
   }
   // K rounds, and one more where the border matters; sub-lane k keeps the winner of round k
-  uint32_t taken = 0, border = 0;
-  int owner_of = 0;
-  const int rounds = __all_sync(kAll, exact) ? cfg.K : cfg.K + 1;
+  uint32_t won = 0, next = 0;
+  const int rounds = exact ? cfg.K : cfg.K + 1;
   for (int k = 0; k < rounds; ++k) {
-    const uint32_t winner = sub_max<L>(key[0] | kPlaceBits);
-    const int owner = lowest_lane(sub_ballot<L>((key[0] | kPlaceBits) == winner));   // lowest index of a tie
-    border = winner;
-    const uint32_t head = __shfl_sync(kAll, key[0], owner, L);
-    if (lane == k) {
-      taken = head;
-      owner_of = owner;
-    }
-    if (lane == owner) {
+    const uint32_t winner = sub_max<L>(key[0]);
+    if (lane == k) won = winner;
+    if (lane == k - 1) next = winner;
+    if (key[0] == winner) {
 #pragma unroll
       for (int j = 0; j + 1 < P; ++j) key[j] = key[j + 1];
       key[P - 1] = 0u;
     }
   }
-  const uint32_t won = taken | kPlaceBits;
-  const uint32_t below = __shfl_down_sync(kAll, won, 1, L);
-  const uint32_t next = lane == cfg.K - 1 ? border : below;
-  if (!exact && lane < cfg.K && next > (kNoneKey | kPlaceBits)) {
-    if (biased) {
-      const float x = K::value(won & ~kPlaceBits), y = K::value(next & ~kPlaceBits);
-      close |= x - y <= 2.0f * kScoreError * (unit + fabsf(x));
-    } else {
-      close |= won == next;
-    }
-  }
-  const bool empty = lane < cfg.K && won <= (kNoneKey | kPlaceBits);
+  if (!exact && lane < cfg.K && next) close |= (won >> 8) - (next >> 8) <= unsure;
+  const bool empty = lane < cfg.K && won == 0;
   const unsigned unfilled = sub_ballot<L>(empty);
   const bool nothing = (unfilled & 1u) != 0;   // a row whose mask leaves nothing: the lowest indices with weight 0
   const unsigned undecided = sub_ballot<L>(close);   // by every lane: not behind a condition that rows differ in
   bool settled = nothing || (undecided == 0 && unfilled == 0);
-  *expert = nothing ? lane : owner_of * P + static_cast<int>(kPlaceBits - (taken & kPlaceBits));
+  *expert = nothing ? lane : static_cast<int>(255u - (won & 255u));
   float w = 0.0f;
   if (lane < cfg.K && settled && !nothing) {
     const float x = load(*expert);
