@@ -191,7 +191,7 @@ int bind_int8(B200MoePlan& p) {
           }
         }
     int smem = 0;
-    g.stages = i8_stages(g.boxes, p.token_tile, g.split, &smem);
+    g.stages = i8_stages(first_box == 2, first_box == 2 && p.gather, g.boxes, p.token_tile, g.split, &smem);
     const long long items = most * ((g.n_out + (first_box == 2 ? 128 : 128 * g.boxes) - 1) / (first_box == 2 ? 128 : 128 * g.boxes));
     g.grid = static_cast<int>(g.split > 1 ? items * g.split : items < p.num_sms ? items : p.num_sms);
   };

@@ -13,6 +13,11 @@
 // product: the two accumulators are two neighbouring tiles of 128 channels (256 channels per tile share every row), or
 // with one box per stage the even and the odd K steps of one tile of 128 channels, added in the epilogue.
 //
+// Epilogue: the accumulator has the channel on the lane, so a warp that stored what it holds would write 64 bytes of each
+// row per instruction, two per lane. It passes 16 rows of its 32 channels through 2 KB of shared memory of its own and
+// writes 16 bytes per lane. Without gathering, four more warps share the work: with 256-row tiles the accumulators
+// take all of tensor memory and nothing hides the epilogue.
+//
 // kSplit: few tiles for the SMs there are. A thread-block cluster works on one tile, each CTA on a slice of K; the
 // int32 partial sums meet through distributed shared memory (exact, so the split changes no bit either) and every CTA
 // finishes some of the rows.
@@ -38,16 +43,15 @@ namespace {
 using namespace ptx;
 using namespace tile;
 
-constexpr int kThreads = 224;
+constexpr int kThreads = 224;   // warps 0 .. 6
 constexpr int kMmaWarpB = 6;
 constexpr int kGatherWarps = 4;
-constexpr int kGatherThreads = kThreads + 32 * kGatherWarps;
+constexpr int kMaxThreads = kThreads + 32 * kGatherWarps;   // warps 7-10 gather, or drain accumulators as warps 2-5 do
 constexpr int kMaxStages = 12;
 constexpr int kRowBytes = 128;                       // K bytes of a stage
 constexpr uint32_t kBoxBytes = kTileM * kRowBytes;   // one weight box, 16 KB
-constexpr int kCtrlBytes = 8192;
+constexpr int kCtrlBytes = 4096;
 constexpr int kMaxTile = 256;
-constexpr int kSplitSmem = kSmemLimit;
 constexpr int kMaxSplit = 8;
 
 struct Ctrl {
@@ -58,7 +62,6 @@ struct Ctrl {
   uint64_t drain[2];
   uint32_t tmem_base;
   int abort;
-  alignas(16) float row_scale[4][kMaxTile];   // of the tile an epilogue warp works on, a copy per warp
   Tables tables;
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block too large");
@@ -66,6 +69,44 @@ static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block too large");
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+
+// What an epilogue warp has in shared memory, behind Ctrl.
+template <typename Out>
+struct EpilogueWarp {
+  static constexpr int kPitch = 32 * sizeof(Out) + 16;   // padding against bank conflicts
+  alignas(16) float row_scale[kMaxTile];                 // of the tile it works on
+  alignas(16) unsigned char transpose[16 * kPitch];      // 16 rows of its 32 channels
+};
+constexpr int epilogue_warps(bool gather, bool split) { return split ? 0 : gather ? 4 : 8; }
+constexpr int ctrl_bytes(bool gate_up, bool gather, bool split) {
+  return kCtrlBytes + epilogue_warps(gather, split) *
+                          static_cast<int>(gate_up ? sizeof(EpilogueWarp<float>) : sizeof(EpilogueWarp<__half>));
+}
+
+// Rows 0 .. 15 (of which `rows` exist) of 32 channels from channel0: v[j] is row j of channel channel0 + lane. `dst` is
+// row 0; `buffer` is this warp's own. Rows that start on 16 bytes are written in pieces of 16 bytes.
+template <typename Out>
+__device__ __forceinline__ void store_rows(Out* dst, const float (&v)[16], int rows, int channel0, int n_out,
+                                           unsigned char* buffer, int lane) {
+  constexpr int kTransposePitch = EpilogueWarp<Out>::kPitch;
+  constexpr int kPiece = 16 / sizeof(Out), kPerRow = 32 / kPiece;   // values per piece, pieces per row
+  if (n_out % kPiece == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    __syncwarp();   // the rows before are read
+#pragma unroll
+    for (int j = 0; j < 16; ++j) store_out(reinterpret_cast<Out*>(buffer + j * kTransposePitch) + lane, v[j]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16 * kPerRow / 32; ++i) {
+      const int row = i * (32 / kPerRow) + lane / kPerRow, channel = channel0 + (lane % kPerRow) * kPiece;
+      const uint4 piece = *reinterpret_cast<const uint4*>(buffer + row * kTransposePitch + (lane % kPerRow) * 16);
+      if (row < rows && channel < n_out) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(row) * n_out + channel) = piece;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < rows && channel0 + lane < n_out) store_out(dst + static_cast<size_t>(j) * n_out + channel0 + lane, v[j]);
+  }
+}
 
 __device__ __forceinline__ float scaled(uint32_t sum, float scale) { return static_cast<float>(static_cast<int>(sum)) * scale; }
 __device__ __forceinline__ float swiglu(float gate, float up) { return (gate / (1.0f + __expf(-gate))) * up; }
@@ -84,17 +125,16 @@ __device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr, uint32_t cta) {
 // kGateUp: SwiGLU epilogue (Out = float, two boxes). kGather: token rows through source_rows. kBoxes: weight boxes (tiles
 // of 128 channels) per stage. kSplit: one tile per cluster, K split over its CTAs.
 template <bool kGateUp, bool kGather, int kBoxes, bool kSplit, typename Out>
-__global__ void __launch_bounds__(kGather || kSplit ? kGatherThreads : kThreads, 1)
+__global__ void __launch_bounds__(kMaxThreads, 1)
 grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
-  constexpr int kBlock = kGather || kSplit ? kGatherThreads : kThreads;   // a split product without gathering has four
-                                                                          // warps that only help with the partial sums
+  constexpr int kEpilogueWarps = kGather || kSplit ? 4 : 8;
   static_assert(!kGateUp || kBoxes == 2, "gate and up are the two boxes");
   constexpr int kTileChannels = kGateUp ? kTileM : kBoxes * kTileM;
   constexpr uint32_t kWBytes = kBoxes * kBoxBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Ctrl* c = reinterpret_cast<Ctrl*>(smem_raw);
   const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t stage_off = ((raw_addr + kCtrlBytes + 1023u) & ~1023u) - raw_addr;
+  const uint32_t stage_off = ((raw_addr + ctrl_bytes(kGateUp, kGather, kSplit) + 1023u) & ~1023u) - raw_addr;
   unsigned char* stages = smem_raw + stage_off;
   const int token_tile = g.token_tile, num_stages = g.stages;
   const uint32_t stage_bytes = kWBytes + static_cast<uint32_t>(token_tile) * kRowBytes;
@@ -112,7 +152,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&c->tmem_full[a], 2);
-      mbar_init(&c->tmem_empty[a], 4);   // one arrival per epilogue warp
+      mbar_init(&c->tmem_empty[a], kEpilogueWarps);   // one arrival each
       mbar_init(&c->drain[a], 1);
     }
     c->abort = 0;
@@ -279,9 +319,11 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");   // never leave with copies in flight
-  } else if (warp < kMmaWarpB) {
+  } else if (warp < kMmaWarpB || kEpilogueWarps == 8) {
     // ------------------------------------------------------------------ epilogue warps
-    const int quarter = warp & 3;
+    const int quarter = warp & 3;                      // the TMEM lane quarter this warp may read
+    const int team = warp < kMmaWarpB ? 0 : 1;         // of the two warps of a quarter
+    EpilogueWarp<Out>* mine = reinterpret_cast<EpilogueWarp<Out>*>(smem_raw + kCtrlBytes) + team * 4 + quarter;
     int acc = 0;
     uint32_t acc_phase = 0;
     if (!kSplit) pdl_wait();   // row scales and output
@@ -294,8 +336,8 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       const float sa = !kSplit && ok_a ? scales[channel] : 0.0f;
       const float sb = !kSplit && ok_b ? scales[kGateUp ? g.n_out + channel : channel_b] : 0.0f;
       // the tile's row scales while its MMAs still run: fetched chunk by chunk they cost two L2 round trips per 16 rows
-      float* row_scale = c->row_scale[quarter];
-      if (!kSplit)
+      float* row_scale = mine->row_scale;
+      if constexpr (!kSplit)
         for (int n = lane; n < t.n_eff; n += 32)
           row_scale[n] = n < t.rows ? g.row_scale[kGather ? g.source_rows[t.row0 + n] : t.row0 + n] : 0.0f;
       if (!__all_sync(0xffffffffu, mbar_wait(&c->tmem_full[acc], acc_phase, &c->abort, g.status))) break;
@@ -318,30 +360,36 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
         }
       } else {
         Out* dst = static_cast<Out*>(g.out) + static_cast<size_t>(t.row0) * g.n_out;
-        for (int n0 = 0; n0 < t.n_eff; n0 += 16) {
+        // this team's part: one of the two boxes, or every other 16 rows
+        constexpr bool kByBox = !kGateUp && kBoxes == 2 && kEpilogueWarps == 8;
+        constexpr int kTeams = kEpilogueWarps / 4;
+        for (int n0 = kByBox ? 0 : team * 16; n0 < t.n_eff; n0 += kByBox ? 16 : 16 * kTeams) {
           uint32_t a[16], b[16];
-          tmem_ld16(taddr + n0, a);
-          tmem_ld16(taddr + token_tile + n0, b);
+          if (kByBox) {
+            tmem_ld16(taddr + (team ? token_tile : 0) + n0, a);
+          } else {
+            tmem_ld16(taddr + n0, a);
+            tmem_ld16(taddr + token_tile + n0, b);
+          }
           float scale[16];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<float4*>(scale + 4 * j) = *reinterpret_cast<const float4*>(row_scale + n0 + 4 * j);
           tmem_ld_wait();
+          float v[16];
+          const float s_mine = kByBox && team ? sb : sa;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const int n = n0 + j;
-            const float s = scale[j];
-            if (n < t.rows) {
-              Out* row = dst + static_cast<size_t>(n) * g.n_out;
-              if constexpr (kGateUp) {
-                if (ok_a) store_out(row + channel, swiglu(scaled(a[j], s * sa), scaled(b[j], s * sb)));
-              } else if constexpr (kBoxes == 2) {
-                if (ok_a) store_out(row + channel, scaled(a[j], s * sa));
-                if (ok_b) store_out(row + channel_b, scaled(b[j], s * sb));
-              } else {
-                if (ok_a) store_out(row + channel, scaled(a[j] + b[j], s * sa));
-              }
-            }
+            if constexpr (kGateUp) v[j] = swiglu(scaled(a[j], scale[j] * sa), scaled(b[j], scale[j] * sb));
+            else if constexpr (kBoxes == 1) v[j] = scaled(a[j] + b[j], scale[j] * sa);
+            else v[j] = scaled(a[j], scale[j] * s_mine);
+          }
+          const int channel0 = (kByBox && team ? channel_b : channel) - lane;
+          store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel0, g.n_out, mine->transpose, lane);
+          if constexpr (!kGateUp && kBoxes == 2 && !kByBox) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = scaled(b[j], scale[j] * sb);
+            store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel_b - lane, g.n_out, mine->transpose, lane);
           }
         }
       }
@@ -368,7 +416,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       // a unit is one row of one box (gate/up: of both); units go round the CTAs, then the warps
       const int units = (kBoxes == 2 && !kGateUp ? 2 : 1) * t.rows;
       for (int u = static_cast<int>(cta) + static_cast<int>(ctas) * warp; u < units;
-           u += static_cast<int>(ctas) * kBlock / 32) {
+           u += static_cast<int>(ctas) * kMaxThreads / 32) {
         const int n = u % t.rows, box = u / t.rows;
         const int channel = t.ct * kTileChannels + box * kTileM + lane * 4;
         const float row_scale = g.row_scale[kGather ? g.source_rows[t.row0 + n] : t.row0 + n];
@@ -419,10 +467,10 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
 template <bool kGateUp, bool kGather, int kBoxes, bool kSplit, typename Out>
 cudaError_t launch(const I8Gemm& g, cudaStream_t s) {
   int smem = 0;
-  i8_stages(g.boxes, g.token_tile, g.split, &smem);
+  i8_stages(kGateUp, kGather, g.boxes, g.token_tile, g.split, &smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(g.grid);
-  cfg.blockDim = dim3(kGather || kSplit ? kGatherThreads : kThreads);
+  cfg.blockDim = dim3(kMaxThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -445,14 +493,14 @@ cudaError_t launch_product(const I8Gemm& g, cudaStream_t s) {
 
 }  // namespace
 
-int i8_stages(int boxes, int token_tile, int split, int* smem_bytes) {
+int i8_stages(bool gate_up, bool gather, int boxes, int token_tile, int split, int* smem_bytes) {
   const int stage = boxes * static_cast<int>(kBoxBytes) + token_tile * kRowBytes;
   // the partial sums of a split tile take the place of the drained stages
   const int partial = split > 1 ? boxes * token_tile * kTileM * 4 : 0;
-  const int space = (split > 1 ? kSplitSmem : kSmemLimit) - kCtrlBytes - 1024;
-  int stages = space / stage;
+  const int ctrl = ctrl_bytes(gate_up, gather, split > 1) + 1024;
+  int stages = (kSmemLimit - ctrl) / stage;
   if (stages > kMaxStages) stages = kMaxStages;
-  *smem_bytes = kCtrlBytes + 1024 + (stages * stage > partial ? stages * stage : partial);
+  *smem_bytes = ctrl + (stages * stage > partial ? stages * stage : partial);
   return stages;
 }
 
@@ -466,7 +514,7 @@ double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxe
   const long long tiles = row_tiles * ((n_out + 128 * boxes - 1) / (128 * boxes));
   const int blocks = (k + kRowBytes - 1) / kRowBytes;
   int smem = 0;
-  if (i8_stages(boxes, token_tile, split, &smem) < 2 || smem > kSmemLimit) return -1.0;
+  if (i8_stages(false, false, boxes, token_tile, split, &smem) < 2 || smem > kSmemLimit) return -1.0;
   const double bytes = boxes * static_cast<double>(kBoxBytes) + token_tile * kRowBytes;
   double block = bytes / 50.0;
   if (block < boxes * 2.0 * token_tile) block = boxes * 2.0 * token_tile;

@@ -54,7 +54,7 @@ struct I8Gemm {
   int split;                   // CTAs of a cluster that share a tile's K; 1: persistent CTAs, a tile each
   int grid;
 };
-int i8_stages(int boxes, int token_tile, int split, int* smem_bytes);
+int i8_stages(bool gate_up, bool gather, int boxes, int token_tile, int split, int* smem_bytes);
 // Cycles that a product of `row_tiles` tiles of `token_tile` rows with n_out channels and k values would take in the
 // given form, or -1 where the form does not exist. See grouped_gemm_i8.cu.
 double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxes, int split, int sms);
