@@ -221,6 +221,28 @@ int launch_int8_gate_up(const B200MoePlan& p, cudaStream_t s) {
   return check_cuda(e, "gate_up launch");
 }
 
+int launch_int8_small(const B200MoePlan& p, bool gate_up, cudaStream_t s) {
+  const B200MoeShape& sh = p.shape;
+  const B200MoeBuffers& b = p.buf;
+  LayerSmall a{};
+  a.x = gate_up ? b.x : b.activated;
+  a.weight = static_cast<const int8_t*>(gate_up ? b.gate_up : b.down);
+  a.w_scale = static_cast<const float*>(gate_up ? b.gate_up_scales : b.down_scales);
+  a.y = gate_up ? b.activated : b.down_output;
+  a.q = static_cast<int8_t*>(gate_up ? b.x_q : b.activated_q);
+  a.q_scale = static_cast<float*>(gate_up ? b.x_scale : b.activated_scale);
+  a.ids = b.ids;
+  a.mapping = static_cast<const int*>(b.mapping);
+  a.ids_are_int64 = sh.ids_are_int64;
+  a.experts = sh.experts;
+  a.topk = sh.topk;
+  a.routes = p.routes;
+  a.k = gate_up ? sh.hidden : sh.intermediate;
+  a.n_out = gate_up ? sh.intermediate : sh.hidden;
+  a.w_rows = gate_up ? 2 * sh.intermediate : sh.hidden;
+  return check_cuda(launch_layer_small(a, gate_up, p.num_sms, s), gate_up ? "gate_up launch" : "down launch");
+}
+
 int launch_int8_down(const B200MoePlan& p, cudaStream_t s) {
   QuantizeRows q{};
   q.x = p.buf.activated;
@@ -445,7 +467,8 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   w.token_tile = tile;
   w.schedule = schedule;
   w.launches = s.tokens == 0 ? 0 : (s.use_router ? 1 : 0) + (p->dispatch_fused ? 2 : 3) + (s.route_only ? 0 : 3);
-  if (is_int8(s) && s.tokens) w.launches += 2;       // x and the activated rows are quantised
+  p->int8_small = is_int8(s) && !s.token_tile && layer_small_serves(s.tokens, s.topk, s.hidden, s.intermediate);
+  if (is_int8(s) && s.tokens && !p->int8_small) w.launches += 2;       // x and the activated rows are quantised
   if (s.route_only == 2) w.launches -= 1;            // no row copy
   if ((p->gather || is_int8(s)) && p->dispatch_fused && s.tokens) w.launches -= 1;  // no row copy kernel
   if (s.external_dispatch) w.launches = s.tokens == 0 ? 0 : 2;  // gate_up + down only
@@ -657,6 +680,7 @@ static int gate_up_stage(B200MoePlan* p, void* stream, bool chained) {
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->schedule != B200MOE_SCHEDULE_TCGEN05) return check_cuda(launch_gate_up_generic(*p, s), "gate_up launch");
+  if (p->int8_small) return launch_int8_small(*p, true, s);
   if (is_int8(p->shape)) return launch_int8_gate_up(*p, s);
   // W4: up to 16 rows per tile the weights are dequantised in registers (weight-streaming kernel); above, the
   // dequantised operand goes to tensor memory while two accumulator sets still fit beside it (tile <= 64), to
@@ -678,6 +702,7 @@ static int down_stage(B200MoePlan* p, void* stream, bool chained) {
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->schedule != B200MOE_SCHEDULE_TCGEN05) return check_cuda(launch_down_generic(*p, s), "down launch");
+  if (p->int8_small) return launch_int8_small(*p, false, s);
   if (is_int8(p->shape)) return launch_int8_down(*p, s);
   if (is_w4(p->shape.down_format)) {
     if (w4r_serves(*p)) return check_cuda(launch_down_w4r(*p, s, chained), "down launch");

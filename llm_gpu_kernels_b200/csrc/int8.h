@@ -35,6 +35,21 @@ struct LinearSmall {
 bool linear_small_serves(int tokens, int k, int n);
 cudaError_t launch_linear_small(const LinearSmall& a, cudaStream_t s);
 
+// One of the two products of a layer for a few routes (layer_small.cu), which quantises its rows itself.
+struct LayerSmall {
+  const void* x;             // gate/up: BF16 rows of the tokens; down: FP32 rows in grouped order
+  const int8_t* weight;
+  const float* w_scale;
+  void* y;                   // gate/up: FP32 [routes, n_out]; down: BF16; both in grouped order
+  int8_t* q;                 // the quantised rows and their scales, for whoever reads the workspace
+  float* q_scale;
+  const void* ids;
+  const int* mapping;
+  int ids_are_int64, experts, topk, routes, k, n_out, w_rows;
+};
+bool layer_small_serves(int tokens, int topk, int hidden, int intermediate);
+cudaError_t launch_layer_small(const LayerSmall& a, bool gate_up, int sms, cudaStream_t s);
+
 // One grouped product in int8 (grouped_gemm_i8.cu). Rows of group e are offsets[e] .. + counts[e] of the activations, or
 // without `tasks` all `rows` of them belong to the one group there is.
 struct I8Gemm {

@@ -68,7 +68,6 @@ int b200moe_linear_create(const B200MoeLinearShape* shape, B200MoeLinear** out) 
   p->shape = *shape;
   p->small = linear_small_serves(shape->tokens, shape->k, shape->n);
   choose_tiles(p);
-  if (shape->reserved[0]) p->token_tile = shape->reserved[0], p->boxes = shape->reserved[1], p->split = shape->reserved[2], p->small = false;
   *out = p;
   return B200MOE_OK;
 }

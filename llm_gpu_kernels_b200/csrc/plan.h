@@ -51,6 +51,7 @@ struct B200MoePlan {
   int w4r_stages_down = 0, w4r_smem_down = 0;
   // INT8 plans: the two products; no BF16 rows are grouped
   bool int8 = false;
+  bool int8_small = false;   // a few routes: products without tensor cores (layer_small.cu)
   b200moe::I8Gemm i8_gate_up{}, i8_down{};
 };
 

@@ -380,6 +380,12 @@ def check_layer(p, x, gate_up, down, ids, rw):
 LAYER = [
     # tokens, experts, topk, hidden, inter, pattern, token tile
     (1, 1, 1, 16, 16, "random", 0), (1, 8, 2, 256, 128, "random", 0), (2, 3, 2, 67, 33, "random", 0),
+    # one token of up to 8 routes and two of up to 2 without tensor cores, and the same with a pinned tile, which is with
+    # them
+    (1, 8, 2, 256, 128, "random", 16), (2, 3, 2, 67, 33, "random", 16), (1, 9, 9, 72, 40, "random", 0), (2, 9, 3, 72, 40, "random", 0),
+    (1, 8, 8, 2100, 1030, "random", 0),
+    (4, 4, 4, 520, 2050, "random", 0), (16, 16, 2, 24, 1, "random", 0), (31, 2, 1, 1, 40, "random", 0), (32, 4, 1, 40, 17, "all_hot", 0),
+    (33, 4, 1, 40, 17, "all_hot", 0),
     (17, 16, 4, 128, 96, "random", 0), (40, 8, 2, 256, 128, "random", 16), (40, 8, 2, 256, 128, "all_hot", 0),
     (33, 5, 3, 200, 130, "last_hot", 32), (64, 4, 2, 520, 264, "random", 64), (130, 4, 4, 128, 384, "random", 128),
     (300, 2, 1, 384, 256, "random", 256), (97, 32, 4, 1000, 72, "hot", 0), (50, 64, 8, 72, 40, "duplicate", 0),
