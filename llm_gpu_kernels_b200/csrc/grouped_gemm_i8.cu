@@ -508,8 +508,9 @@ int i8_stages(bool gate_up, bool gather, int boxes, int token_tile, int split, i
 // all but four within 12 %). A stage takes the longest of its bytes at 50 bytes per cycle out of L2, its MMAs (half a
 // cycle per row and K step of 32) and 210 cycles of hand-over; a tile that is not followed by another on its SM shows
 // its epilogue, 36 cycles per row and box; adding up a split tile takes 3200 cycles and 38 per row and box. Above 512
-// columns of accumulators there is only one set and every epilogue shows: 128 x 2 boxes in 25 rounds were faster than
-// 256 x 2 in 13 (393 and 451 us, 8192 x 4096 x 14336), so such tiles are for a single round only.
+// columns of accumulators there is only one set and every epilogue shows, at 30 cycles per row and box with eight warps:
+// 128 x 2 boxes is faster while K is short (8192 x 1024 x 4096: 54 and 66 us), 256 x 2 once K is long, where the power
+// limit decides and a third less goes through L2 (8192 x 4096 x 14336, back to back for seconds: 442 and 421 us).
 double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxes, int split, int sms) {
   const long long tiles = row_tiles * ((n_out + 128 * boxes - 1) / (128 * boxes));
   const int blocks = (k + kRowBytes - 1) / kRowBytes;
@@ -525,7 +526,7 @@ double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxe
     return (blocks + split - 1) / split * block + 3200.0 + 38.0 * rows;
   }
   const double rounds = static_cast<double>((tiles + sms - 1) / sms);
-  if (rounds > 1 && 4 * token_tile > 512) return -1.0;
+  if (rounds > 1 && 4 * token_tile > 512) return rounds * (blocks * block + 30.0 * rows);
   return rounds * blocks * block + 36.0 * rows;
 }
 
