@@ -140,9 +140,9 @@ typedef struct {
   size_t scratch;       /* dispatch partial histograms, router flag, tile counter and per-expert completion
                            counters of the chained GEMM kernels */
   size_t source_rows;   /* [R] int32: token whose row each grouped row is (inverse of mapping; 0 unless gathers) */
-  size_t x_q;           /* INT8 plans: [T, H rounded up to 16] int8, x quantised row by row (plans that do not gather:
-                           [R, ..], in grouped order); else 0 */
-  size_t x_scale;       /* INT8 plans: [T] or [R] float32 */
+  size_t x_q;           /* INT8 plans: [R, H rounded up to 16] int8, the routes' rows of x, quantised, in grouped order;
+                           else 0 */
+  size_t x_scale;       /* INT8 plans: [R] float32 */
   size_t activated_q;   /* INT8 plans: [R, I rounded up to 16] int8 */
   size_t activated_scale; /* INT8 plans: [R] float32 */
   int32_t token_tile;   /* resolved tile */

@@ -161,8 +161,6 @@ int bind_int8(B200MoePlan& p) {
   gu.w_scale = static_cast<const float*>(b.gate_up_scales);
   gu.row_scale = static_cast<const float*>(b.x_scale);
   gu.out = b.activated;
-  gu.x_q = static_cast<const int8_t*>(b.x_q);
-  gu.source_rows = p.gather ? static_cast<const int*>(b.source_rows) : nullptr;
   gu.n_out = s.intermediate;
   gu.k = s.hidden;
   gu.w_rows = 2 * s.intermediate;
@@ -181,7 +179,7 @@ int bind_int8(B200MoePlan& p) {
     double best = -1.0;
     if (tiles <= 2 * p.num_sms)
       for (int boxes = first_box; boxes <= 2; ++boxes)
-        for (int split = 1; split <= (first_box == 1 || p.gather ? 8 : 1); split *= 2) {   // a split gate/up gathers
+        for (int split = 1; split <= 8; split *= 2) {
           // gate/up has a channel tile of its own for each of its boxes' 128 channels
           const double c = i8_cycles(most, first_box == 2 ? 2 * g.n_out : g.n_out, g.k, p.token_tile, boxes, split, p.num_sms);
           if (c >= 0.0 && (best < 0.0 || c < best)) {
@@ -191,7 +189,7 @@ int bind_int8(B200MoePlan& p) {
           }
         }
     int smem = 0;
-    g.stages = i8_stages(first_box == 2, first_box == 2 && p.gather, g.boxes, p.token_tile, g.split, &smem);
+    g.stages = i8_stages(first_box == 2, g.boxes, p.token_tile, g.split, &smem);
     const long long items = most * ((g.n_out + (first_box == 2 ? 128 : 128 * g.boxes) - 1) / (first_box == 2 ? 128 : 128 * g.boxes));
     g.grid = static_cast<int>(g.split > 1 ? items * g.split : items < p.num_sms ? items : p.num_sms);
   };
@@ -199,7 +197,7 @@ int bind_int8(B200MoePlan& p) {
   choose(dn, 1);
   const uint64_t E = s.experts, I = s.intermediate, H = s.hidden;
   if ((rc = encode_i8(&gu.tm_w, b.gate_up, E * 2 * I, H, int8_pitch(s.hidden), 128, true))) return rc;
-  if (!p.gather && (rc = encode_i8(&gu.tm_act, b.x_q, p.routes, H, int8_pitch(s.hidden), p.token_tile, false))) return rc;
+  if ((rc = encode_i8(&gu.tm_act, b.x_q, p.routes, H, int8_pitch(s.hidden), p.token_tile, false))) return rc;
   if ((rc = encode_i8(&dn.tm_w, b.down, E * H, I, int8_pitch(s.intermediate), 128, true))) return rc;
   return encode_i8(&dn.tm_act, b.activated_q, p.routes, I, int8_pitch(s.intermediate), p.token_tile, false);
 }
@@ -212,10 +210,8 @@ int launch_int8_gate_up(const B200MoePlan& p, cudaStream_t s) {
   q.rows = p.shape.tokens;
   q.q = static_cast<int8_t*>(p.buf.x_q);
   q.scale = static_cast<float*>(p.buf.x_scale);
-  if (!p.gather) {   // straight into grouped order
-    q.mapping = static_cast<const int*>(p.buf.mapping);
-    q.copies = p.shape.topk;
-  }
+  q.mapping = static_cast<const int*>(p.buf.mapping);   // straight into grouped order
+  q.copies = p.shape.topk;
   cudaError_t e = launch_quantize_rows(q, s);
   if (e == cudaSuccess) e = launch_i8_gate_up(p.i8_gate_up, s);
   return check_cuda(e, "gate_up launch");
@@ -435,9 +431,7 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   p->gather = s.fused_gather && schedule == B200MOE_SCHEDULE_TCGEN05 && !s.route_only && !s.external_dispatch &&
               r > 0 && (!is_w4(s.gate_up_format) || tile <= 16) &&
               (s.fused_gather == 2 || r <= static_cast<long long>(s.experts) * 384);
-  // INT8: no BF16 rows are grouped. The quantised rows are gathered, or past the same three tiles per expert written in
-  // grouped order by the kernel that quantises them.
-  if (is_int8(s)) p->gather = r > 0 && r <= static_cast<long long>(s.experts) * 384;
+  if (is_int8(s)) p->gather = false;   // the kernel that quantises x writes the rows in grouped order
 
   B200MoeWorkspace& w = p->ws;
   const size_t T = s.tokens, H = s.hidden, I = s.intermediate, E = s.experts, R = r;
@@ -455,9 +449,8 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   w.scratch = align256((static_cast<size_t>(p->partitions) * E + blocks + 2 + E) * 4);
   w.source_rows = p->gather ? R * 4 : 0;
   if (is_int8(s)) {
-    const size_t x_rows = p->gather ? T : R;   // one per token, or one per route in grouped order
-    w.x_q = x_rows * int8_pitch(s.hidden);
-    w.x_scale = x_rows * 4;
+    w.x_q = R * int8_pitch(s.hidden);
+    w.x_scale = R * 4;
     w.activated_q = R * int8_pitch(s.intermediate);
     w.activated_scale = R * 4;
   }

@@ -3,9 +3,11 @@
 //
 // The organisation is that of the BF16 kernel (grouped_gemm_tcgen05.cu): weights are the M operand (128 output channels
 // of a group), rows the N operand, N set per tile; one persistent CTA per SM, warp 0 loads by TMA, warps 1 and 6 issue
-// the MMAs of one accumulator each, warps 2-5 drain accumulators, warps 7-10 gather token rows. A k-block is 128 bytes
-// = 128 values: the same bytes per stage as there, twice the products. Sums are exact in 32 bits (k <= 131072), so
-// neither the tile schedule nor the order of K can change a bit of the result.
+// the MMAs of one accumulator each, warps 2-5 and 7-10 drain accumulators. A k-block is 128 bytes = 128 values: the same
+// bytes per stage as there, twice the products. Sums are exact in 32 bits (k <= 131072), so neither the tile schedule nor
+// the order of K can change a bit of the result. Token rows are not gathered here: the kernel that quantises x writes
+// them in grouped order, one byte per value, and a TMA box brings them (gathering them in four warps with cp.async, as
+// the BF16 kernel does: 156 and 151 us for 1024 tokens of 128 experts, 348 and 300 for 4096, 110 and 102 for 193 of 60).
 //
 // gate/up: the two accumulators are the gate and the up rows of the same 128 channels; the epilogue scales both,
 // applies SwiGLU and stores FP32: the down product quantises these rows against their largest value, and rounding
@@ -15,8 +17,8 @@
 //
 // Epilogue: the accumulator has the channel on the lane, so a warp that stored what it holds would write 64 bytes of each
 // row per instruction, two per lane. It passes 16 rows of its 32 channels through 2 KB of shared memory of its own and
-// writes 16 bytes per lane. Without gathering, four more warps share the work: with 256-row tiles the accumulators
-// take all of tensor memory and nothing hides the epilogue.
+// writes 16 bytes per lane. Eight warps share the work: with 256-row tiles the accumulators take all of tensor memory
+// and nothing hides the epilogue.
 //
 // kSplit: few tiles for the SMs there are. A thread-block cluster works on one tile, each CTA on a slice of K; the
 // int32 partial sums meet through distributed shared memory (exact, so the split changes no bit either) and every CTA
@@ -45,8 +47,7 @@ using namespace tile;
 
 constexpr int kThreads = 224;   // warps 0 .. 6
 constexpr int kMmaWarpB = 6;
-constexpr int kGatherWarps = 4;
-constexpr int kMaxThreads = kThreads + 32 * kGatherWarps;   // warps 7-10 gather, or drain accumulators as warps 2-5 do
+constexpr int kMaxThreads = kThreads + 32 * 4;   // warps 7-10 drain accumulators as warps 2-5 do
 constexpr int kMaxStages = 12;
 constexpr int kRowBytes = 128;                       // K bytes of a stage
 constexpr uint32_t kBoxBytes = kTileM * kRowBytes;   // one weight box, 16 KB
@@ -77,9 +78,9 @@ struct EpilogueWarp {
   alignas(16) float row_scale[kMaxTile];                 // of the tile it works on
   alignas(16) unsigned char transpose[16 * kPitch];      // 16 rows of its 32 channels
 };
-constexpr int epilogue_warps(bool gather, bool split) { return split ? 0 : gather ? 4 : 8; }
-constexpr int ctrl_bytes(bool gate_up, bool gather, bool split) {
-  return kCtrlBytes + epilogue_warps(gather, split) *
+constexpr int epilogue_warps(bool split) { return split ? 0 : 8; }
+constexpr int ctrl_bytes(bool gate_up, bool split) {
+  return kCtrlBytes + epilogue_warps(split) *
                           static_cast<int>(gate_up ? sizeof(EpilogueWarp<float>) : sizeof(EpilogueWarp<__half>));
 }
 
@@ -122,19 +123,19 @@ __device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr, uint32_t cta) {
   return v;
 }
 
-// kGateUp: SwiGLU epilogue (Out = float, two boxes). kGather: token rows through source_rows. kBoxes: weight boxes (tiles
-// of 128 channels) per stage. kSplit: one tile per cluster, K split over its CTAs.
-template <bool kGateUp, bool kGather, int kBoxes, bool kSplit, typename Out>
+// kGateUp: SwiGLU epilogue (Out = float, two boxes). kBoxes: weight boxes (tiles of 128 channels) per stage. kSplit: one
+// tile per cluster, K split over its CTAs.
+template <bool kGateUp, int kBoxes, bool kSplit, typename Out>
 __global__ void __launch_bounds__(kMaxThreads, 1)
 grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
-  constexpr int kEpilogueWarps = kGather || kSplit ? 4 : 8;
+  constexpr int kEpilogueWarps = kSplit ? 4 : 8;
   static_assert(!kGateUp || kBoxes == 2, "gate and up are the two boxes");
   constexpr int kTileChannels = kGateUp ? kTileM : kBoxes * kTileM;
   constexpr uint32_t kWBytes = kBoxes * kBoxBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Ctrl* c = reinterpret_cast<Ctrl*>(smem_raw);
   const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t stage_off = ((raw_addr + ctrl_bytes(kGateUp, kGather, kSplit) + 1023u) & ~1023u) - raw_addr;
+  const uint32_t stage_off = ((raw_addr + ctrl_bytes(kGateUp, kSplit) + 1023u) & ~1023u) - raw_addr;
   unsigned char* stages = smem_raw + stage_off;
   const int token_tile = g.token_tile, num_stages = g.stages;
   const uint32_t stage_bytes = kWBytes + static_cast<uint32_t>(token_tile) * kRowBytes;
@@ -147,7 +148,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < num_stages; ++s) {
-      mbar_init(&c->full[s], kGather ? 1 + 32 * kGatherWarps : 1);
+      mbar_init(&c->full[s], 1);
       mbar_init(&c->empty[s], 2);   // the commits of the two MMA issuers
     }
     for (int a = 0; a < 2; ++a) {
@@ -202,7 +203,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       auto load_weights = [&](const Tile& t, int kb, int st) {
         unsigned char* to = stages + static_cast<size_t>(st) * stage_bytes;
         const int w_row = t.expert * g.w_rows + t.ct * kTileChannels;
-        mbar_expect_tx(&c->full[st], kGather ? kWBytes : stage_bytes);
+        mbar_expect_tx(&c->full[st], stage_bytes);
         tma_load_2d(to, &g.tm_w, &c->full[st], kb * kRowBytes, w_row, pol_w);
         if (kBoxes == 2)
           tma_load_2d(to + kBoxBytes, &g.tm_w, &c->full[st], kb * kRowBytes, w_row + (kGateUp ? g.n_out : kTileM), pol_w);
@@ -222,9 +223,8 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
             if (!mbar_wait(&c->empty[stage], phase ^ 1u, &c->abort, g.status)) { ok = false; break; }
             load_weights(t, kb, stage);
           }
-          if (!kGather)
-            tma_load_2d(stages + static_cast<size_t>(stage) * stage_bytes + kWBytes, &g.tm_act, &c->full[stage],
-                        kb * kRowBytes, t.row0, pol_act);
+          tma_load_2d(stages + static_cast<size_t>(stage) * stage_bytes + kWBytes, &g.tm_act, &c->full[stage], kb * kRowBytes,
+                      t.row0, pol_act);
           ++issued;
           if (++stage == num_stages) { stage = 0; phase ^= 1u; }
         }
@@ -255,7 +255,6 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&c->full[stage], phase, &c->abort, g.status)) { ok = false; break; }
           tc_fence_after();
-          if (kGather) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // cp.async-written rows -> MMA
           const uint32_t w_addr = smem_u32(stages + static_cast<size_t>(stage) * stage_bytes);
           const uint32_t a_addr = w_addr + kWBytes;
 #pragma unroll
@@ -278,47 +277,6 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
         mbar_wait_plain(&c->drain[half], 0);
       }
     }
-  } else if (kGather && warp > kMmaWarpB) {
-    // ------------------------------------------------------------------ gather warps: token rows -> activation tile
-    constexpr int kIters = kMaxTile * 8 / (32 * kGatherWarps);   // 16-byte pieces per lane and stage
-    const int gt = (warp - kMmaWarpB - 1) * 32 + lane;
-    const int chunk = gt & 7;
-    const int pitch = int8_pitch(g.k);
-    pdl_wait();
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int item = first_item; ok && item < total_items; item = next_item(item)) {
-      const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
-      const int iters = (t.rows * 8 + 32 * kGatherWarps - 1) / (32 * kGatherWarps);
-      int src[kIters];   // token of row it * 16 + gt / 8, -1 past the tile's rows
-#pragma unroll
-      for (int it = 0; it < kIters; ++it) {
-        const int n = it * 16 + (gt >> 3);
-        src[it] = (it < iters && n < t.rows) ? g.source_rows[t.row0 + n] : -1;
-      }
-      for (int kb = kb0; kb < kb1; ++kb) {
-        int free_ok = 1;
-        if (lane == 0) free_ok = mbar_wait(&c->empty[stage], phase ^ 1u, &c->abort, g.status) ? 1 : 0;
-        free_ok = __shfl_sync(0xffffffffu, free_ok, 0);
-        if (!free_ok) { ok = false; break; }
-        const uint32_t act = smem_u32(stages + static_cast<size_t>(stage) * stage_bytes) + kWBytes;
-        const int k = kb * kRowBytes + chunk * 16;
-        const uint32_t bytes = k < pitch ? 16u : 0u;   // a piece past the row is zero-filled, as TMA does
-#pragma unroll
-        for (int it = 0; it < kIters; ++it) {
-          if (it < iters && src[it] >= 0) {
-            const int n = it * 16 + (gt >> 3);
-            const uint32_t dst = act + static_cast<uint32_t>(n) * 128u + (static_cast<uint32_t>(chunk ^ (n & 7)) << 4);
-            const int8_t* from = g.x_q + static_cast<size_t>(src[it]) * pitch + (bytes ? k : 0);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
-          }
-        }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&c->full[stage])) : "memory");
-        if (++stage == num_stages) { stage = 0; phase ^= 1u; }
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");   // never leave with copies in flight
   } else if (warp < kMmaWarpB || kEpilogueWarps == 8) {
     // ------------------------------------------------------------------ epilogue warps
     const int quarter = warp & 3;                      // the TMEM lane quarter this warp may read
@@ -339,7 +297,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       float* row_scale = mine->row_scale;
       if constexpr (!kSplit)
         for (int n = lane; n < t.n_eff; n += 32)
-          row_scale[n] = n < t.rows ? g.row_scale[kGather ? g.source_rows[t.row0 + n] : t.row0 + n] : 0.0f;
+          row_scale[n] = n < t.rows ? g.row_scale[t.row0 + n] : 0.0f;
       if (!__all_sync(0xffffffffu, mbar_wait(&c->tmem_full[acc], acc_phase, &c->abort, g.status))) break;
       __syncwarp();
       tc_fence_after();
@@ -419,7 +377,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
            u += static_cast<int>(ctas) * kMaxThreads / 32) {
         const int n = u % t.rows, box = u / t.rows;
         const int channel = t.ct * kTileChannels + box * kTileM + lane * 4;
-        const float row_scale = g.row_scale[kGather ? g.source_rows[t.row0 + n] : t.row0 + n];
+        const float row_scale = g.row_scale[t.row0 + n];
         int sum[4] = {}, sum_up[4] = {};
         int4 v[kMaxSplit], w[kGateUp ? kMaxSplit : 1];   // all loads first: one round trip
 #pragma unroll
@@ -464,10 +422,10 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
   }
 }
 
-template <bool kGateUp, bool kGather, int kBoxes, bool kSplit, typename Out>
+template <bool kGateUp, int kBoxes, bool kSplit, typename Out>
 cudaError_t launch(const I8Gemm& g, cudaStream_t s) {
   int smem = 0;
-  i8_stages(kGateUp, kGather, g.boxes, g.token_tile, g.split, &smem);
+  i8_stages(kGateUp, g.boxes, g.token_tile, g.split, &smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(g.grid);
   cfg.blockDim = dim3(kMaxThreads);
@@ -482,22 +440,22 @@ cudaError_t launch(const I8Gemm& g, cudaStream_t s) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kSplit ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, grouped_gemm_i8_kernel<kGateUp, kGather, kBoxes, kSplit, Out>, g);
+  return cudaLaunchKernelEx(&cfg, grouped_gemm_i8_kernel<kGateUp, kBoxes, kSplit, Out>, g);
 }
 
 template <typename Out>
 cudaError_t launch_product(const I8Gemm& g, cudaStream_t s) {
-  if (g.split > 1) return g.boxes == 2 ? launch<false, false, 2, true, Out>(g, s) : launch<false, false, 1, true, Out>(g, s);
-  return g.boxes == 2 ? launch<false, false, 2, false, Out>(g, s) : launch<false, false, 1, false, Out>(g, s);
+  if (g.split > 1) return g.boxes == 2 ? launch<false, 2, true, Out>(g, s) : launch<false, 1, true, Out>(g, s);
+  return g.boxes == 2 ? launch<false, 2, false, Out>(g, s) : launch<false, 1, false, Out>(g, s);
 }
 
 }  // namespace
 
-int i8_stages(bool gate_up, bool gather, int boxes, int token_tile, int split, int* smem_bytes) {
+int i8_stages(bool gate_up, int boxes, int token_tile, int split, int* smem_bytes) {
   const int stage = boxes * static_cast<int>(kBoxBytes) + token_tile * kRowBytes;
   // the partial sums of a split tile take the place of the drained stages
   const int partial = split > 1 ? boxes * token_tile * kTileM * 4 : 0;
-  const int ctrl = ctrl_bytes(gate_up, gather, split > 1) + 1024;
+  const int ctrl = ctrl_bytes(gate_up, split > 1) + 1024;
   int stages = (kSmemLimit - ctrl) / stage;
   if (stages > kMaxStages) stages = kMaxStages;
   *smem_bytes = ctrl + (stages * stage > partial ? stages * stage : partial);
@@ -515,7 +473,7 @@ double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxe
   const long long tiles = row_tiles * ((n_out + 128 * boxes - 1) / (128 * boxes));
   const int blocks = (k + kRowBytes - 1) / kRowBytes;
   int smem = 0;
-  if (i8_stages(false, false, boxes, token_tile, split, &smem) < 2 || smem > kSmemLimit) return -1.0;
+  if (i8_stages(false, boxes, token_tile, split, &smem) < 2 || smem > kSmemLimit) return -1.0;
   const double bytes = boxes * static_cast<double>(kBoxBytes) + token_tile * kRowBytes;
   double block = bytes / 50.0;
   if (block < boxes * 2.0 * token_tile) block = boxes * 2.0 * token_tile;
@@ -533,17 +491,16 @@ double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxe
 int configure_i8() {
   using bf16 = __nv_bfloat16;
   const void* kernels[] = {
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, false, 2, false, float>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, true, 2, false, float>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, true, 2, true, float>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, false, bf16>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, true, bf16>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, false, bf16>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, true, bf16>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, false, __half>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 1, true, __half>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, false, __half>),
-      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, false, 2, true, __half>)};
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, 2, false, float>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<true, 2, true, float>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 1, false, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 1, true, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 2, false, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 2, true, bf16>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 1, false, __half>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 1, true, __half>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 2, false, __half>),
+      reinterpret_cast<const void*>(grouped_gemm_i8_kernel<false, 2, true, __half>)};
   for (const void* kernel : kernels) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (e != cudaSuccess) {
@@ -555,8 +512,7 @@ int configure_i8() {
 }
 
 cudaError_t launch_i8_gate_up(const I8Gemm& g, cudaStream_t s) {
-  if (g.split > 1) return launch<true, true, 2, true, float>(g, s);
-  return g.source_rows != nullptr ? launch<true, true, 2, false, float>(g, s) : launch<true, false, 2, false, float>(g, s);
+  return g.split > 1 ? launch<true, 2, true, float>(g, s) : launch<true, 2, false, float>(g, s);
 }
 
 cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, cudaStream_t s) {

@@ -54,27 +54,25 @@ cudaError_t launch_layer_small(const LayerSmall& a, bool gate_up, int sms, cudaS
 // without `tasks` all `rows` of them belong to the one group there is.
 struct I8Gemm {
   CUtensorMap tm_w;            // int8 [groups * w_rows, k], rows int8_pitch(k) bytes apart, box 128 bytes x 128 rows
-  CUtensorMap tm_act;          // int8 [rows, k], box 128 bytes x token_tile rows (not read when gathering)
+  CUtensorMap tm_act;          // int8 [rows, k], box 128 bytes x token_tile rows
   const float* w_scale;        // [groups * w_rows]
-  const float* row_scale;      // [rows]; gathering: [tokens]
+  const float* row_scale;      // [rows]
   void* out;                   // gate/up: float [rows, n_out]; else [rows, n_out] of out_dtype
   const int* offsets;
   const int* counts;
   const int* tasks;
   int* status;
-  const int* source_rows;      // gathering: token of each row; else null
-  const int8_t* x_q;           // gathering: [tokens, int8_pitch(k)]
   int groups, rows, n_out, k, w_rows, token_tile, stages, stream_weights;
   int boxes;                   // tiles of 128 channels per stage (gate/up: 2)
   int split;                   // CTAs of a cluster that share a tile's K; 1: persistent CTAs, a tile each
   int grid;
 };
-int i8_stages(bool gate_up, bool gather, int boxes, int token_tile, int split, int* smem_bytes);
+int i8_stages(bool gate_up, int boxes, int token_tile, int split, int* smem_bytes);
 // Cycles that a product of `row_tiles` tiles of `token_tile` rows with n_out channels and k values would take in the
 // given form, or -1 where the form does not exist. See grouped_gemm_i8.cu.
 double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxes, int split, int sms);
 int configure_i8();   // opt-in shared memory of the kernels on the current device
-cudaError_t launch_i8_gate_up(const I8Gemm& g, cudaStream_t s);   // gathers if source_rows is set
+cudaError_t launch_i8_gate_up(const I8Gemm& g, cudaStream_t s);
 cudaError_t launch_i8_product(const I8Gemm& g, int out_dtype, cudaStream_t s);
 // 2-D int8 tensor map, box 128 bytes x box_rows, 128-byte swizzle, zero fill past the ends.
 int encode_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows,

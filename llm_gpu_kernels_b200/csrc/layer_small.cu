@@ -68,14 +68,14 @@ layer_small_kernel(const LayerSmall a) {
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) bits = max(bits, part[i]);
   const RowScale scale = row_scale_of(bits);
-  const bool keep = blockIdx.x == 0 && (!kGateUp || route % a.topk == 0);   // one block per row leaves it in memory too
-  if (keep && threadIdx.x == 0) a.q_scale[row] = scale.scale;
+  const bool keep = blockIdx.x == 0;   // one block per route leaves its row in memory too, in grouped order
+  if (keep && threadIdx.x == 0) a.q_scale[at] = scale.scale;
   for (int k = threadIdx.x * 8; k < smem_pitch; k += kThreads * 8) {
     float v[8] = {};
     load8<T, kVec>(x, k, a.k, v);
     const uint2 q = quantize8<sizeof(T) == 2>(v, scale);
     *reinterpret_cast<uint2*>(smem + k) = q;
-    if (keep && k < pitch) *reinterpret_cast<uint2*>(a.q + static_cast<size_t>(row) * pitch + k) = q;
+    if (keep && k < pitch) *reinterpret_cast<uint2*>(a.q + static_cast<size_t>(at) * pitch + k) = q;
   }
   __syncthreads();
   for (; n < a.n_out; n += step) {

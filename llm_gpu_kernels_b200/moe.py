@@ -325,9 +325,8 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             source_rows=int32((r,)) if sizes.gathers else None)
         if int8:
             byte = lambda rows, size: torch.empty((rows, size // max(1, rows)), device=device, dtype=torch.int8)
-            x_rows = tokens if sizes.gathers else r
-            plan.x_q, plan.activated_q = byte(x_rows, sizes.x_q), byte(r, sizes.activated_q)
-            plan.x_scale = torch.empty((x_rows,), device=device, dtype=torch.float32)
+            plan.x_q, plan.activated_q = byte(r, sizes.x_q), byte(r, sizes.activated_q)
+            plan.x_scale = torch.empty((r,), device=device, dtype=torch.float32)
             plan.activated_scale = torch.empty((r,), device=device, dtype=torch.float32)
         for name, tensor in (workspace or {}).items():  # caller-provided workspace (peer-visible buffers)
             if tuple(tensor.shape) != tuple(getattr(plan, name).shape) or tensor.dtype != getattr(plan, name).dtype:
