@@ -1,6 +1,8 @@
 // Rows to 8-bit integers in memory (the formula and its rounding: int8_rows.cuh).
 // Bound by memory: it reads a row once (up to 32 values per thread stay in registers between the maximum and the
-// rounding) and writes a byte per value; at a serving batch by launch latency.
+// rounding) and writes a byte per value; at a serving batch by launch latency. Six or seven instructions per value
+// keep it from the copy rate where rows are many: 1024 x 2048 BF16 5.5 us, 8192 x 4096 BF16 23 us (4.4 TB/s, issue slots
+// 69 %), 8192 x 768 FP32 10.4 us (3.0 TB/s).
 #include "int8.h"
 #include "int8_rows.cuh"
 #include "pdl.cuh"

@@ -22,8 +22,9 @@
 // the end by K lanes at once, from logits read again, so full-precision exp and division cost one instruction sequence
 // per row. 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups (5.4 us would be the HBM floor): 80 us with unsorted
 // keys and per-expert weights (1930 warp instructions per row), 47 us with sorted keys that leave ties and experts to
-// ballots (910), 41 us like this (895 instructions for a row that FP32 settles: 33 us if all did). Sixteen experts per lane and two rows per warp need as many instructions per row (the
-// warp-wide redux of 32 lanes becomes four shuffles) and more registers: 73 us.
+// ballots (910), 41 us like this (895 instructions for a row that FP32 settles: 33 us if all did). Sixteen experts per
+// lane and two rows per warp need as many instructions per row (the warp-wide redux of 32 lanes becomes four shuffles)
+// and more registers: 73 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
