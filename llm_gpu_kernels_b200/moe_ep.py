@@ -79,8 +79,7 @@ class CudaBackend:
         tile = token_tile_for(global_routes, experts, 1) if tensor_tiles else 0
         self.expert_plan = _prepare(self.recv_x, gate_up_local, down_local, self.recv_ids, self.recv_rw,
                                     token_tile=tile, valid_routes=self.valid,
-                                    gate_up_scales=gate_up_scales, down_scales=down_scales, router=router,
-                                 router_bias=router_bias)
+                                    gate_up_scales=gate_up_scales, down_scales=down_scales)
         self.local_experts = local_experts
 
     # token-owning side

@@ -368,3 +368,64 @@ def test_routing_feeds_a_layer(dev):
     routing.run()
     assert torch.equal(layer.run(), whole.run())
     assert torch.equal(routing.ids, ids) and torch.equal(routing.routing_weights, rw)
+
+
+def _one_rank(rank, port, score):
+    """A configured router in both expert-parallel layers on one rank, against the layer on one GPU."""
+    import os
+    import torch.distributed as dist
+    from llm_gpu_kernels_b200.moe_ep import prepare_ep_moe, prepare_peer_ep_moe
+    from llm_gpu_kernels_b200.moe_ranked import prepare_ranked_moe_launcher
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), NCCL_NVLS_ENABLE="0")
+    torch.cuda.set_device(0)
+    dev = torch.device("cuda", 0)
+    dist.init_process_group("nccl", rank=0, world_size=1, device_id=dev)
+    try:
+        t, e, k, h, i = 50, 16, 4, 128, 64
+        g = torch.Generator().manual_seed(5)
+        draw = lambda *shape: (torch.randn(*shape, generator=g) * 0.1).bfloat16().to(dev)
+        x, wr, gate_up, down = draw(t, h), draw(e, h), draw(e, 2 * i, h), draw(e, h, i)
+        how = dict(router_weight=wr, router=RouterConfig(score=score, groups=4, kept_groups=2, scale=2.5),
+                   router_bias=torch.linspace(-0.2, 0.2, e, device=dev))
+        routes = lambda: (torch.zeros(t, k, dtype=torch.int32, device=dev), torch.zeros(t, k, device=dev))
+        ids, weights = routes()
+        ep = prepare_ep_moe(x, gate_up, down, ids, weights, experts=e, **how)
+        tile = ep.backend.expert_plan
+        ids1, weights1 = routes()
+        single = prepare_ranked_moe_launcher(x, gate_up, down, ids1, weights1, token_tile=tile.token_tile,
+                                             down_tiles=tile.down_tiles, **how)
+        expected = single.run()
+        out = ep.run()
+        assert torch.equal(ids, ids1) and torch.equal(weights, weights1) and torch.equal(out, expected)
+        ids2, weights2 = routes()
+        peer = prepare_peer_ep_moe(x, gate_up, down, ids2, weights2, experts=e, **how)
+        try:
+            out = peer.run()
+            torch.cuda.synchronize()
+            peer.check_inputs()
+            assert torch.equal(ids2, ids1) and torch.equal(weights2, weights1) and torch.equal(out, expected)
+        finally:
+            peer.close()
+    finally:
+        dist.destroy_process_group()
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_configured_router_expert_parallel(score):
+    torch.multiprocessing.spawn(_one_rank, args=(29747, score), nprocs=1, join=True)
+
+
+def test_expert_side_has_no_router(monkeypatch):
+    """Only the plan that owns the tokens routes: the plan of the local experts gets no router arguments."""
+    from types import SimpleNamespace
+    from llm_gpu_kernels_b200 import moe_ep
+    calls = []
+    monkeypatch.setattr(moe_ep, "_prepare", lambda *args, **kw: calls.append(kw) or SimpleNamespace())
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    how = dict(router_weight=torch.zeros(8, 64), router=RouterConfig(score="sigmoid"), router_bias=torch.zeros(8))
+    moe_ep.CudaBackend(x, torch.zeros(8, 128, 64), torch.zeros(8, 64, 64), torch.zeros(4, 2), torch.zeros(4, 2),
+                       experts=8, capacity=8, global_routes=8, **how)
+    token, expert = calls
+    assert all(token[name] is value for name, value in how.items())
+    assert not any(name in expert and expert[name] is not None for name in how)
