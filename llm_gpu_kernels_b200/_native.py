@@ -189,9 +189,16 @@ def check(code: int):
     raise RuntimeError(f"b200moe error {code}: {message}")
 
 
-def launch(call, args, device):
-    """``call(args, stream)`` on the current stream of device ``device``; ``args`` is a struct or a plan handle. Kept
-    short: for one token the kernels behind it take less time than this function."""
+def tracing():
+    """Something records or replaces PyTorch operators (torch.compile, export, make_fx, a dispatch mode): calls of the
+    library must be visible to it as operators."""
+    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+
+
+def launch(call, args, device, written):
+    """``call(args, stream)`` on the current stream of device ``device``; ``args`` is a struct or a plan handle. The
+    tensors ``written`` count as modified in place, so that autograd refuses a backward pass through values that were
+    overwritten. Kept short: for one token the kernels behind it take less time than this function."""
     arg = ctypes.byref(args) if isinstance(args, ctypes.Structure) else args
     if torch._C._cuda_getDevice() == device:
         code = call(arg, torch._C._cuda_getCurrentRawStream(device))
@@ -200,6 +207,7 @@ def launch(call, args, device):
             code = call(arg, torch.cuda.current_stream().cuda_stream)
     if code:
         check(code)
+    torch.autograd.graph.increment_version(written)
 
 
 def _span(t):

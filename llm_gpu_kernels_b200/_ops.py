@@ -90,7 +90,7 @@ def route(logits: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor,
                                     renormalize=int(renormalize), scale=scale),
         logits=rows.data_ptr(), bias=bias.data_ptr() if bias is not None else None, ids=ids.data_ptr(),
         weights=routing_weights.data_ptr())
-    _native.launch(_native.load().b200moe_route, args, rows.device.index)
+    _native.launch(_native.load().b200moe_route, args, rows.device.index, ())   # the operator declares what it writes
 
 
 @route.register_fake
@@ -103,12 +103,15 @@ def int8_linear(plan: int, x: torch.Tensor, weight: torch.Tensor, weight_scale: 
                 x_q: torch.Tensor, x_scale: torch.Tensor, status: torch.Tensor) -> None:
     """One product of the prepared plan (``b200moe_linear_forward``) for tracers. The kernels use the addresses bound at
     prepare time; where a tracer passes copies, values are copied in and out as for ``forward``."""
-    prepared = _LINEARS[plan]()
+    owner = _LINEARS.get(plan)
+    prepared = owner() if owner is not None else None
+    if prepared is None:
+        raise RuntimeError("int8 product: its prepared object is gone")
     if x.shape[0] == 0:
         return
     if x.data_ptr() != prepared.x.data_ptr():
         prepared.x.copy_(x)
-    _native.launch(prepared._call, prepared._plan, prepared._device)
+    _native.launch(prepared._call, prepared._plan, prepared._device, ())
     for given, real in ((output, prepared.output), (x_q, prepared.x_q), (x_scale, prepared.x_scale),
                         (status, prepared.status)):
         if given.data_ptr() != real.data_ptr():

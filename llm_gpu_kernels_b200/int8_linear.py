@@ -37,11 +37,11 @@ class PreparedInt8Linear:
 
     def run(self):
         """One product on the current stream; returns ``output``."""
-        if torch.compiler.is_compiling():
+        if _native.tracing():
             _ops.int8_linear(self._plan.value, self.x, self.weight.storage, self.weight.scales, self.output, self.x_q,
                              self.x_scale, self.status)
         elif self.x.shape[0]:
-            _native.launch(self._call, self._plan, self._device)
+            _native.launch(self._call, self._plan, self._device, (self.output, self.x_q, self.x_scale, self.status))
         return self.output
 
     def check(self):

@@ -110,6 +110,7 @@ class PreparedMoE:
     _plan: object = field(default=None, repr=False)
     _forward: object = field(default=None, repr=False)
     _op_args: tuple = field(default=None, repr=False)
+    _written: tuple = field(default=None, repr=False)
 
     @property
     def workspace_bytes(self):
@@ -155,8 +156,9 @@ class PreparedMoE:
         self._stage(4)
 
     def run(self):
-        """One forward on the current stream (``b200moe_forward``). While ``torch.compile`` traces, the call goes through
-        the registered PyTorch operator ``torch.ops.b200moe.forward``, which tells the tracer what it writes."""
+        """One forward on the current stream (``b200moe_forward``). While ``torch.compile`` or another tracer records,
+        the call goes through the registered PyTorch operator ``torch.ops.b200moe.forward``, which tells the tracer
+        what it writes."""
         if self.x.shape[0] == 0:
             return self.output
         if self._op_args is None:
@@ -170,12 +172,13 @@ class PreparedMoE:
                 workspace.append(self.source_rows)
             workspace += self.int8_workspace()
             self._op_args = (self._plan.value, self.x, weights, self.ids, self.routing_weights, self.output, workspace)
+            self._written = (self.ids, self.routing_weights, self.output, *workspace)
             _ops.register_plan(self)
-        if torch.compiler.is_compiling():
+        if _native.tracing():
             _ops.forward(*self._op_args)
         else:
             # the same call without the operator's dispatch, which takes longer than a small forward
-            _native.launch(self._forward, self._plan, self.x.device.index)
+            _native.launch(self._forward, self._plan, self.x.device.index, self._written)
         return self.output
 
     def __del__(self):

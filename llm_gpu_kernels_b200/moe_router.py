@@ -93,12 +93,12 @@ class PreparedRouting:
 
     def run(self):
         """Routes every row on the current stream; returns (ids, routing_weights)."""
-        if torch.compiler.is_compiling():
+        if _native.tracing():
             c = self.config
             _ops.route(self.logits, self.bias, self.ids, self.routing_weights, SCORES[c.score], c.groups, c.kept,
                        GROUP_SCORES[c.group_score], c.renormalize, float(c.scale))
         elif self.logits.shape[0]:
-            _native.launch(self._call, self._args, self._device)
+            _native.launch(self._call, self._args, self._device, (self.ids, self.routing_weights))
         return self.ids, self.routing_weights
 
 

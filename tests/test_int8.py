@@ -515,3 +515,48 @@ def test_router_experts_and_shared_product_together(dev, t, h):
     # one more BF16 rounding than the layer alone: that of the shared product
     off = torch.linalg.norm(layer.base.output.cpu().double() - exact) / torch.linalg.norm(exact)
     assert off <= 4 * 2.0 ** -8 + 1e-3, off
+
+
+# ---- what PyTorch learns of a run
+def prepared_of_each_kind(dev):
+    from llm_gpu_kernels_b200.moe_router import prepare_routing
+    from llm_gpu_kernels_b200.moe_ranked import prepare_ranked_moe_launcher
+    x, gate_up, down, ids, rw = layer_inputs(20, 8, 2, 128, 64, "random", dev)
+    layer = prepare_int8_moe(x, gate_up, down, ids, rw)
+    plain = prepare_ranked_moe_launcher(x, gate_up.dequantize().bfloat16(), down.dequantize().bfloat16(), ids, rw)
+    linear = prepare_int8_linear(x, Int8Weight(gate_up.values[0], gate_up.scales[0]))
+    routing = prepare_routing(torch.randn(20, 8, device=dev), 2)
+    return [("forward", layer.run, layer.base.output), ("forward", plain.run, plain.base.output),
+            ("int8_linear", linear.run, linear.output), ("route", routing.run, routing.routing_weights)]
+
+
+@gpu
+def test_run_counts_as_a_change_in_place(dev):
+    """A result that autograd saved and a later run overwrote may not give a gradient in silence."""
+    for name, run, result in prepared_of_each_kind(dev):
+        run()
+        factor = torch.ones(result.shape, device=dev, requires_grad=True, dtype=result.dtype)
+        (result * factor).sum().backward()
+        assert torch.equal(factor.grad, result), name
+        loss = (result * factor).sum()
+        run()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+@gpu
+def test_dispatch_modes_see_the_operators(dev):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    for name, run, result in prepared_of_each_kind(dev):
+        want = result.clone()
+        seen = []
+        result.zero_()
+        with Names():
+            run()
+        assert f"b200moe::{name}" in seen and torch.equal(result, want)
