@@ -103,6 +103,14 @@ int b200moe_linear_bind(B200MoeLinear* p, const B200MoeLinearBuffers* b) {
       set_error("linear: null buffer");
       return B200MOE_ERR_INVALID;
     }
+  const void* read[] = {b->x, b->weight, b->weight_scale};
+  const void* written[] = {b->output, b->x_q, b->x_scale, b->status};
+  for (const void* in : read)
+    for (const void* to : written)
+      if (in == to) {
+        set_error("linear: a written buffer aliases an input");
+        return B200MOE_ERR_INVALID;
+      }
   if (s.tokens > 1 && b->x_pitch < s.k) {
     set_error("linear: row pitch %lld of x is smaller than k=%d", static_cast<long long>(b->x_pitch), s.k);
     return B200MOE_ERR_INVALID;

@@ -209,7 +209,11 @@ def _validate(x, gate_up, down, ids, routing_weights, router_weight, gate_up_sca
         e, h, intermediate = int(route_only_experts), x.shape[1], 64
         gate_up_shape = (e, 2 * intermediate, h)
         gate_up = down = None
-    elif isinstance(gate_up, Int8Weight):
+    elif isinstance(gate_up, Int8Weight) or isinstance(down, Int8Weight):
+        if not isinstance(gate_up, Int8Weight) or not isinstance(down, Int8Weight):
+            raise TypeError("gate_up and down must both be Int8Weight or neither")
+        if gate_up.values.ndim != 3 or down.values.ndim != 3 or gate_up_scales is not None or down_scales is not None:
+            raise ValueError("8-bit experts: Int8Weight [E,2I,H] and [E,H,I] without other scales required")
         gate_up_shape = tuple(gate_up.shape)
         e, h, intermediate = down.shape
     elif gate_up_scales is None:

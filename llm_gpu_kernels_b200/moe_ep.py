@@ -28,6 +28,7 @@ from dataclasses import dataclass
 import torch
 import torch.distributed as dist
 
+from .int8_weights import Int8Weight
 from .moe import _prepare
 from .moe_full_policy import token_tile_for
 
@@ -56,6 +57,11 @@ def received_expert_ids(recv_counts: torch.Tensor, total: int):
     peers, local = recv_counts.shape
     pattern = torch.arange(local, dtype=torch.int32, device=recv_counts.device).repeat(peers)
     return torch.repeat_interleave(pattern, recv_counts.reshape(-1).long(), output_size=total)
+
+
+def _no_int8(*weights):
+    if any(isinstance(w, Int8Weight) for w in weights):
+        raise TypeError("expert parallelism takes BF16 or packed 4-bit experts, not Int8Weight")
 
 
 class CudaBackend:
@@ -187,6 +193,7 @@ def prepare_ep_moe(x, gate_up_local, down_local, ids, routing_weights, *, expert
     ``capacity`` = rows this rank can receive
     (default: every route of every rank, assuming equal token counts).
     """
+    _no_int8(gate_up_local, down_local)
     world = dist.get_world_size(group)
     rank = dist.get_rank(group)
     lo, hi = expert_range(rank, world, experts)
@@ -274,6 +281,7 @@ class PeerExpertParallelMoE:
         import ctypes
         from . import _native
         from .moe import _prepare_expert_side
+        _no_int8(gate_up_local, down_local)
         self._native = _native
         self.lib = _native.load()
         self.group = group

@@ -71,7 +71,7 @@ def test_linear_workspace_and_state():
                 x_scale=0x60000, status=0x70000)
     for bad in (dict(x=None), dict(weight=None), dict(output=None), dict(x_q=None), dict(status=None), dict(x_pitch=66),
                 dict(weight=0x20008), dict(x_q=0x50008), dict(x=0x10001), dict(output=0x40001), dict(x_scale=0x60002),
-                dict(weight_scale=0x30001), dict(status=0x70002)):
+                dict(weight_scale=0x30001), dict(status=0x70002), dict(output=0x10000), dict(x_q=0x20000)):
         assert lib.b200moe_linear_bind(handle, ctypes.byref(_native.LinearBuffers(**{**good, **bad}))) == _native.ERR_INVALID
     assert lib.b200moe_linear_forward(handle, None) == _native.ERR_STATE
     lib.b200moe_linear_destroy(handle)
@@ -477,6 +477,11 @@ def test_layer_refuses(dev):
             prepare_int8_moe(*args)
     with pytest.raises(ValueError):
         prepare_int8_moe(x, gate_up, down, ids, rw, token_tile=48)
+    from llm_gpu_kernels_b200.moe_ranked import prepare_ranked_moe_launcher
+    plain = lambda w: w.dequantize().bfloat16()
+    for args in ((x, gate_up, plain(down), ids, rw), (x, plain(gate_up), down, ids, rw)):
+        with pytest.raises(TypeError, match="both be Int8Weight"):
+            prepare_ranked_moe_launcher(*args)
 
 
 @gpu
@@ -560,3 +565,13 @@ def test_dispatch_modes_see_the_operators(dev):
         with Names():
             run()
         assert f"b200moe::{name}" in seen and torch.equal(result, want)
+
+
+def test_expert_parallelism_refuses():
+    from llm_gpu_kernels_b200.moe_ep import prepare_ep_moe, prepare_peer_ep_moe
+    gate_up, down = quantize_int8(torch.ones(4, 64, 32)), quantize_int8(torch.ones(4, 32, 32))
+    x, ids, rw = torch.ones(2, 32).bfloat16(), torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, 2)
+    for prepare in (prepare_ep_moe, prepare_peer_ep_moe):
+        for weights in ((gate_up, down), (gate_up, torch.ones(4, 32, 32)), (torch.ones(4, 64, 32), down)):
+            with pytest.raises(TypeError, match="not Int8Weight"):
+                prepare(x, *weights, ids, rw, experts=4)
