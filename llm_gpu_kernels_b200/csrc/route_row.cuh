@@ -156,7 +156,8 @@ __device__ __noinline__ void route_exact(const Config& cfg, const float* __restr
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     const float b = bias != nullptr && lane * P + j < cfg.E ? bias[lane * P + j] : 0.0f;
-    const double c = bias != nullptr ? score_of(cfg, v[j], top, sum) + static_cast<double>(b) : v[j];
+    // + 0: zeros of both signs tie
+    const double c = bias != nullptr ? score_of(cfg, v[j], top, sum) + static_cast<double>(b) : v[j] + 0.0;
     key[j] = v[j] > none && b > -INFINITY ? K::of(c) : 0ull;   // false for NaN
     place[j] = j;
   }
@@ -330,7 +331,8 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
   bool close = false;
   if (exact) {
 #pragma unroll
-    for (int j = 0; j < P; ++j) key[j] = c[j] > none ? (K::of(c[j]) & ~255u) | (255u - (lane * P + j)) : 0u;
+    for (int j = 0; j < P; ++j)   // + 0: zeros of both signs tie
+      key[j] = c[j] > none ? (K::of(c[j] + 0.0f) & ~255u) | (255u - (lane * P + j)) : 0u;
   } else {
     float low = INFINITY, high = none;
 #pragma unroll

@@ -189,6 +189,20 @@ def test_ties_go_to_the_lower_index(dev):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("config", [{}, dict(score="sigmoid"), dict(groups=8, kept_groups=3),
+                                    dict(groups=8, kept_groups=3, group_score="top2"), dict(groups=3, kept_groups=2)])
+def test_zeros_of_both_signs_tie(dev, dtype, config):
+    g = torch.Generator().manual_seed(13)
+    experts = 96 if config.get("groups") == 3 else 64
+    logits = torch.where(torch.rand(50, experts, generator=g) < 0.5, -0.0, 0.0)
+    logits[25:] = torch.where(torch.rand(25, experts, generator=g) < 0.8, logits[25:], -1.0 - torch.rand(25, experts, generator=g))
+    logits = logits.to(dtype).to(dev)
+    p = prepare_routing(logits, 6, config=RouterConfig(**config))
+    agree(p.ids, p.routing_weights, logits, 6, **config)
+
+
+@gpu
 def test_extreme_logits(dev):
     """Infinities, the type's lowest value as a mask, and scores that leave the range of FP32."""
     inf, low = math.inf, torch.finfo(torch.float32).min
