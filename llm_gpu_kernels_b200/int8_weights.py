@@ -57,7 +57,7 @@ class Int8Weight:
 
 def quantize_int8(weight: torch.Tensor) -> Int8Weight:
     """Quantise a BF16 / FP16 / FP32 weight [N,K] or [E,N,K] channel by channel, on the device it is on."""
-    if (not isinstance(weight, torch.Tensor) or weight.ndim not in (2, 3)
+    if (not isinstance(weight, torch.Tensor) or weight.ndim not in (2, 3) or 0 in weight.shape
             or weight.dtype not in (torch.bfloat16, torch.float16, torch.float32)):
         raise ValueError("expected a BF16/FP16/FP32 weight [N,K] or [E,N,K]")
     parts = weight if weight.ndim == 3 else weight[None]

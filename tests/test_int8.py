@@ -575,3 +575,9 @@ def test_expert_parallelism_refuses():
         for weights in ((gate_up, down), (gate_up, torch.ones(4, 32, 32)), (torch.ones(4, 64, 32), down)):
             with pytest.raises(TypeError, match="not Int8Weight"):
                 prepare(x, *weights, ids, rw, experts=4)
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (4, 0), (2, 0, 4), (2, 4, 0), (0, 4, 4)])
+def test_quantize_int8_refuses_empty(shape):
+    with pytest.raises(ValueError):
+        quantize_int8(torch.zeros(shape))
