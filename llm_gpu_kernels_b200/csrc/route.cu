@@ -69,7 +69,7 @@ route_kernel(const T* __restrict__ logits, long long pitch, const float* __restr
   const long long first = row * cfg.K;
   const route::Out out{ids_are_int64 ? static_cast<void*>(static_cast<long long*>(ids) + first)
                                      : static_cast<void*>(static_cast<int*>(ids) + first), weights + first, ids_are_int64};
-  route::route_row<P, L>(cfg, l, b, bias, lane, live, [&](int e) { return to_float(row_logits[e]); }, out);
+  route::route_row<P, L>(cfg, l, b, bias, lane, live, [row_logits](int e) { return to_float(row_logits[e]); }, out);
 }
 
 template <typename T, int P, int L>

@@ -12,9 +12,13 @@
 // nobody can fill get the lowest indices not chosen yet, with weight 0, so the ids stay valid for the dispatch.
 //
 // Precision: the weights are FP32. The CHOICE is that of exact arithmetic: where c comes from exp() in FP32, two
-// values closer than the error bound of that computation could be in the wrong order, so a row in which two
-// neighbours of the order (or the groups at the border) are that close is routed again in FP64 (route_exact): one row
-// in a thousand for random logits.
+// values closer than the error bound of that computation could be in the wrong order. Where two neighbours of the order
+// (or the groups at the border) are that close, one row in a thousand for random logits, the experts found (the two
+// largest of each group) are put in order by their c in FP64, one expert per lane (exact_order, exact_groups). That is
+// enough if the next expert is not close as well; otherwise, and in rows with fewer experts left than slots, the whole
+// row is routed in FP64 (route_exact). That pass takes 9 us for a row, most of it instruction fetches, and a single
+// late row shows in the call: with it alone 32768 rows x 256 experts took 41.5 us instead of 35.5, 4099 x 160 masked
+// 11.5 instead of 7.5.
 //
 // What bounds the common pass (route_fast) at many rows is the number of instructions per row, so it keeps the experts
 // of a lane as sorted 32-bit keys that hold the expert too: sorting eight is 19 compare-exchanges of two integer min /
@@ -22,9 +26,9 @@
 // the end by K lanes at once, from logits read again, so full-precision exp and division cost one instruction sequence
 // per row. 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups (5.4 us would be the HBM floor): 80 us with unsorted
 // keys and per-expert weights (1930 warp instructions per row), 47 us with sorted keys that leave ties and experts to
-// ballots (910), 41 us like this (895 instructions for a row that FP32 settles: 33 us if all did). Sixteen experts per
-// lane and two rows per warp need as many instructions per row (the warp-wide redux of 32 lanes becomes four shuffles)
-// and more registers: 73 us.
+// ballots (910), 35.5 us like this (930 instructions for a row that FP32 settles: 34.3 us if all did). Sixteen experts
+// per lane and two rows per warp need as many instructions per row (the warp-wide redux of 32 lanes becomes four
+// shuffles) and more registers: 73 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -133,7 +137,7 @@ __device__ __forceinline__ unsigned long long sub_max64(unsigned long long v) {
 // kept short as well: sorted keys as in route_fast, whole-warp reductions.
 template <int P, int L, typename Load>
 __device__ __noinline__ void route_exact(const Config& cfg, const float* __restrict__ bias, int lane, bool wanted,
-                                         const Load& load, const Out& out) {
+                                         Load load, Out out) {
   using K = Key<double>;
   using KeyT = K::type;
   const double none = -INFINITY;
@@ -276,7 +280,71 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[P]) {
           if (i + j + d < P && (i + j) / (2 * p) == (i + j + d) / (2 * p)) exchange(k[i + j], k[i + j + d]);
 }
 
-// Returns false when FP32 cannot settle the row; otherwise slot `lane` < K of the row is `expert` with weight `w`.
+// c (by_score: the score) of one expert per lane in FP64, as route_exact has it. One small function for every place that
+// needs it, and no loop unrolled: the rare pass runs out of a cold instruction cache.
+template <int P, int L, typename Load>
+__device__ __noinline__ double exact_choice(const Config& cfg, const float* __restrict__ bias, int lane, int expert,
+                                            bool by_score, Load load) {
+  auto logit = [&](int e) { return e < cfg.E ? fmaxf(load(e), -INFINITY) : -INFINITY; };   // NaN -> -inf
+  const double x = logit(expert);
+  if (bias == nullptr && !by_score) return x + 0.0;
+  double top = -INFINITY, sum = 1.0;
+  if (!cfg.sigmoid) {
+    float high = -INFINITY;
+#pragma unroll 1
+    for (int j = 0; j < P; ++j) high = fmaxf(high, logit(lane * P + j));
+    top = Key<float>::value(sub_max<L>(Key<float>::of(high)));
+    sum = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < P; ++j) sum += score_of(cfg, logit(lane * P + j), top, 1.0);
+    sum = sub_sum<L>(sum);
+  }
+  const double s = score_of(cfg, x, top, sum);
+  return bias != nullptr && expert < cfg.E ? s + static_cast<double>(bias[expert]) : s;
+}
+
+// Whether the group of this lane is kept, decided in FP64. a, second: the two largest keys of the lane's group of
+// `lanes` lanes.
+template <int P, int L, typename Load>
+__device__ __noinline__ bool exact_groups(const Config& cfg, const float* __restrict__ bias, int lane, int lanes,
+                                          uint32_t a, uint32_t second, bool by_score, Load load) {
+  const double va = exact_choice<P, L>(cfg, bias, lane, 255 - (a & 255u), by_score, load);
+  const double vb = exact_choice<P, L>(cfg, bias, lane, 255 - (second & 255u), by_score, load);
+  double value = a ? va : -INFINITY;
+  if (second) value = cfg.group_top2 ? va + vb : max(va, vb);
+  int before = 0;
+#pragma unroll 1
+  for (int g = 0; g < cfg.groups; ++g) {
+    const double v = __shfl_sync(kAll, value, g * lanes, L);
+    before += v > value || (v == value && (g + 1) * lanes <= lane);
+  }
+  return before < cfg.kept;
+}
+
+// The candidates of lanes 0 .. K in the order of FP64; lane k gets the k-th.
+template <int P, int L, typename Load>
+__device__ __noinline__ uint32_t exact_order(const Config& cfg, const float* __restrict__ bias, int lane, uint32_t won,
+                                             Load load) {
+  const int expert = 255 - static_cast<int>(won & 255u);
+  const double c = exact_choice<P, L>(cfg, bias, lane, expert, false, load);
+  int before = 0;
+#pragma unroll 1
+  for (int i = 0; i <= cfg.K; ++i) {
+    const double v = __shfl_sync(kAll, c, i, L);
+    const uint32_t other = __shfl_sync(kAll, won, i, L);
+    before += other != 0 && (won == 0 || v > c || (v == c && 255 - static_cast<int>(other & 255u) < expert));
+  }
+  uint32_t mine = 0;
+#pragma unroll 1
+  for (int i = 0; i <= cfg.K; ++i) {
+    const uint32_t other = __shfl_sync(kAll, won, i, L);
+    if (__shfl_sync(kAll, before, i, L) == lane && other != 0) mine = other;
+  }
+  return mine;
+}
+
+// Returns false when FP32 and a look at the candidates in FP64 cannot settle the row; otherwise slot `lane` < K of the
+// row is `expert` with weight `w`.
 // l[j]: logits of experts lane*P + j, b[j]: biases.
 //
 // Keys are (q << 8) | (255 - expert): the larger key has the larger q, or the lower index at equal q, so every key is
@@ -285,11 +353,12 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[P]) {
 // else gives its place between the smallest and the largest c of the row (values below -1e30 count as the smallest):
 // q = 1 + (c - base) * scale, monotonic in c and off by less than 2 from rounding.
 template <int P, int L, typename Load>
-__device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], const float (&b)[P], bool biased, int lane,
-                                           const Load& load, int* expert, float* weight) {
+__device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], const float (&b)[P], int lane,
+                                           const float* __restrict__ bias, Load load, int* expert, float* weight) {
   using K = Key<float>;
+  const bool biased = bias != nullptr;
   const float none = -INFINITY;
-  const bool grouped = cfg.kept < cfg.groups;
+  const bool grouped = L >= 16 && cfg.kept < cfg.groups;   // fewer lanes route without groups only (route.cu)
   float top = none;
   uint32_t low_bits = 0;
 #pragma unroll
@@ -398,6 +467,17 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       // two values of two c each (or scores, whose logits are off by `step`)
       const float far = by_score ? 4.0f * (2e-6f * unit + step) : 2.0f * step * static_cast<float>(unsure + 2u) + 2.4e-7f * fabsf(border);
       close = border - next <= far;   // infinities compare false
+      if (__any_sync(kAll, close)) {
+        // In FP64 from the two largest of each group. They have to be certain: no third one close to the second.
+        int near = 0;
+#pragma unroll
+        for (int j = 0; j < P; ++j) near += key[j] != 0 && (exact ? key[j] >= second : (key[j] >> 8) + unsure >= second >> 8);
+        for (int o = 1; o < lanes; o <<= 1) near += __shfl_xor_sync(kAll, near, o);
+        const bool certain = sub_ballot<L>(near > 2) == 0;
+        const bool exactly = exact_groups<P, L>(cfg, bias, lane, lanes, a, second, by_score, load);
+        if (close) kept = exactly;
+        close = close && !certain;
+      }
     }
     if (!kept) {
 #pragma unroll
@@ -417,7 +497,17 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       key[P - 1] = 0u;
     }
   }
-  if (!exact && lane < cfg.K && next) close |= (won >> 8) - (next >> 8) <= unsure;
+  if (!exact) {
+    const bool tight = lane < cfg.K && next && (won >> 8) - (next >> 8) <= unsure;
+    if (__any_sync(kAll, tight)) {
+      // In FP64 among the K + 1 found, if they are certain: the one after them is not close to the last.
+      const uint32_t after = sub_max<L>(key[0]);
+      const unsigned uncertain = sub_ballot<L>(cfg.K >= L || (lane == cfg.K && after && (won >> 8) - (after >> 8) <= unsure));
+      const uint32_t order = exact_order<P, L>(cfg, bias, lane, won, load);
+      if (uncertain == 0) won = order;
+      else close |= tight;
+    }
+  }
   const bool empty = lane < cfg.K && won == 0;
   const unsigned unfilled = sub_ballot<L>(empty);
   const bool nothing = (unfilled & 1u) != 0;   // a row whose mask leaves nothing: the lowest indices with weight 0
@@ -446,15 +536,15 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
 // do not end at lane borders with a power of two of lanes each go through the general pass.
 template <int P, int L, typename Load>
 __device__ __forceinline__ void route_row(const Config& cfg, float (&l)[P], const float (&b)[P],
-                                          const float* __restrict__ bias, int lane, bool live, const Load& load,
-                                          const Out& out) {
+                                          const float* __restrict__ bias, int lane, bool live, Load load,
+                                          Out out) {
   const int size = cfg.size, lanes = size / P;
   const bool lane_groups = cfg.kept == cfg.groups || (size % P == 0 && (lanes & (lanes - 1)) == 0);
   bool settled = false;
   if (lane_groups) {
     int expert;
     float w;
-    settled = route_fast<P, L>(cfg, l, b, bias != nullptr, lane, load, &expert, &w);
+    settled = route_fast<P, L>(cfg, l, b, lane, bias, load, &expert, &w);
     if (live && settled && lane < cfg.K) out.put(cfg, lane, expert, w);
   }
   if (__any_sync(kAll, live && !settled)) route_exact<P, L>(cfg, bias, lane, live && !settled, load, out);

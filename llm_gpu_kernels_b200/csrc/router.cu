@@ -89,7 +89,7 @@ router_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __r
     for (int j = 0; j < 8; ++j) row[j] = lane * 8 + j < E ? l[lane * 8 + j] : -INFINITY;
     route::load_bias<8>(cfg, bias, lane, b);
     const size_t o = static_cast<size_t>(t0 + warp) * K;
-    route::route_row<8, 32>(cfg, row, b, bias, lane, true, [&](int e) { return l[e]; },
+    route::route_row<8, 32>(cfg, row, b, bias, lane, true, [l](int e) { return l[e]; },
                             route::Out{ids + o, rw + o, sizeof(IdT) == 8});
     return;
   }

@@ -164,7 +164,7 @@ router_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
       const int r = static_cast<int>(cta_rank) * rows_per_cta + rr;
       if (r >= rows_live) break;
       if constexpr (kGeneral) {
-        auto logit = [&](int e) {
+        auto logit = [=](int e) {
           float sum_parts = 0.0f;
           for (int sidx = 0; sidx < ksplit; ++sidx) {  // fixed order: slice 0, 1, ...
             uint32_t remote;

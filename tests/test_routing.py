@@ -179,6 +179,60 @@ def test_scores_closer_than_fp32(dev, score):
 
 
 @gpu
+@pytest.mark.parametrize("experts,topk,biased,config", [
+    (256, 8, True, dict(score="sigmoid", groups=8, kept_groups=4, group_score="top2")),
+    (256, 8, True, dict(score="sigmoid", groups=8, kept_groups=3)),
+    (256, 8, False, dict(score="sigmoid", groups=8, kept_groups=4, group_score="top2")),
+    (160, 6, True, dict(groups=8, kept_groups=3, renormalize=False)),
+    (160, 6, False, dict(groups=8, kept_groups=2, group_score="top2")),
+    (128, 8, True, dict(groups=4, kept_groups=2, group_score="top2")),
+    (256, 8, True, {}), (128, 16, True, dict(score="sigmoid")), (64, 6, True, {}), (32, 4, True, dict(score="sigmoid")),
+    (64, 8, False, {}), (200, 7, False, dict(score="sigmoid")), (16, 15, True, {}), (8, 8, True, dict(score="sigmoid")),
+])
+def test_a_few_close_choices(dev, experts, topk, biased, config):
+    """Rows in which two or three experts, or two groups, are closer than FP32 can tell and the others are not."""
+    g = torch.Generator().manual_seed(experts + topk)
+    rows, groups = 240, config.get("groups", 1)
+    size = experts // groups
+    logits = (1.5 * torch.randn(rows, experts, generator=g)).double()
+    bias = 0.1 * torch.randn(size, generator=g).repeat(groups) if biased else None
+    score = torch.sigmoid if config.get("score") == "sigmoid" else lambda x: torch.softmax(x, -1)
+    nudge = lambda: float(torch.randint(-2, 3, (1,), generator=g)) * 2.0 ** -24
+    for r in range(rows):
+        if r % 3 == 0 and groups > 1:            # two groups alike but for the last bits
+            a, b = torch.randperm(groups, generator=g)[:2].tolist()
+            logits[r, b * size:(b + 1) * size] = logits[r, a * size:(a + 1) * size]
+            top = b * size + int(logits[r, b * size:(b + 1) * size].argmax())
+            logits[r, top] += nudge() * abs(logits[r, top])
+        if r % 3 != 1:
+            continue
+        c = score(logits[r]) + bias if biased else logits[r]
+        order = c.argsort(descending=True)
+        at = int(torch.randint(0, min(topk + 1, experts - 1), (1,), generator=g))
+        for other in order[at + 1:at + 2 + r % 2].tolist():   # raised until it is level with the one at place `at`
+            first = int(order[at])
+            if not biased:
+                logits[r, other] = logits[r, first] * (1 + nudge())
+                continue
+            low, high = -30.0, 30.0
+            for _ in range(60):
+                middle = (low + high) / 2
+                trial = logits[r].clone()
+                trial[other] = middle
+                s = score(trial)
+                if s[other] + bias[other] < s[first] + bias[first]:
+                    low = middle
+                else:
+                    high = middle
+            if -20 < low < 20:
+                logits[r, other] = low * (1 + nudge())
+    logits = logits.float().to(dev)
+    bias = bias.to(dev) if biased else None
+    p = prepare_routing(logits, topk, config=RouterConfig(**config), bias=bias)
+    agree(p.ids, p.routing_weights, logits, topk, bias, **config)
+
+
+@gpu
 def test_ties_go_to_the_lower_index(dev):
     logits = torch.zeros(3, 64, device=dev)
     for bias in (None, torch.zeros(64, device=dev)):
