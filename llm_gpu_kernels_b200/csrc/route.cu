@@ -52,34 +52,36 @@ route_kernel(const T* __restrict__ logits, long long pitch, const float* __restr
   const long long row = live ? wanted : tokens - 1;   // lanes past the end follow the last row and write nothing
   const T* row_logits = logits + row * pitch;
   float l[P], b[P];
-  const bool inside = lane * P < cfg.E;
+  auto logit = [row_logits](int e) { return to_float(row_logits[e]); };
   if (kVec) {
+    int e, count;
+    route::place_of<P, L>(cfg, lane, &e, &count);
+    const bool inside = count > 0;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       l[j] = -INFINITY;
       b[j] = 0.0f;
     }
-    if (inside) load_vec(row_logits + lane * P, l);
-    if (inside && bias != nullptr) load_vec(bias + lane * P, b);
+    if (inside) load_vec(row_logits + e, l);
+    if (inside && bias != nullptr) load_vec(bias + e, b);
   } else {
-#pragma unroll
-    for (int j = 0; j < P; ++j) l[j] = lane * P + j < cfg.E ? to_float(row_logits[lane * P + j]) : -INFINITY;
-    route::load_bias<P>(cfg, bias, lane, b);
+    route::load_row<P, L>(cfg, bias, lane, logit, l, b);
   }
   const long long first = row * cfg.K;
   const route::Out out{ids_are_int64 ? static_cast<void*>(static_cast<long long*>(ids) + first)
                                      : static_cast<void*>(static_cast<int*>(ids) + first), weights + first, ids_are_int64};
-  route::route_row<P, L>(cfg, l, b, bias, lane, live, [row_logits](int e) { return to_float(row_logits[e]); }, out);
+  route::route_row<P, L>(cfg, l, b, bias, lane, live, logit, out);
 }
 
 template <typename T, int P, int L>
-cudaError_t launch(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStream_t s) {
+cudaError_t launch(const B200MoeRouteArgs& a, route::Config cfg, cudaStream_t s) {
+  route::fit(cfg, P, L);
   const T* logits = static_cast<const T*>(a.logits);
   auto* bias = static_cast<const float*>(a.bias);
   auto* w = static_cast<float*>(a.weights);
   constexpr bool kPow2 = (P & (P - 1)) == 0;
   const size_t piece = P * sizeof(T) < 16 ? P * sizeof(T) : 16;
-  const bool vec = kPow2 && cfg.E % P == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
+  const bool vec = kPow2 && (cfg.shift < 0 ? cfg.E : cfg.size) % P == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
                    (a.pitch * sizeof(T)) % piece == 0 && reinterpret_cast<uintptr_t>(bias) % 16 == 0;
   const int rows = kThreads / L;
   const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.tokens) + rows - 1) / rows));
@@ -93,26 +95,27 @@ cudaError_t launch(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStre
 }
 
 // Lanes and experts per lane. Few lanes per row, so that rows share a warp (the instructions of a round are then paid
-// once for several rows), but at least K: a lane per weight. With groups, the first pair that gives every group a power
-// of two of whole lanes; where there is none the kernel takes its general pass.
+// once for several rows), but at least K: a lane per weight. With groups, the fewest experts per lane that leave every
+// group a power of two of whole lanes; where even eight do not (three groups of 70, say) the kernel takes its general
+// pass for every row.
 template <typename T, int L>
 cudaError_t launch_lanes(const B200MoeRouteArgs& a, const route::Config& cfg, cudaStream_t s) {
-  const int size = cfg.size;
+  const bool grouped = cfg.kept < cfg.groups;
   auto fits = [&](int p) {
-    const int lanes = size / p;
-    return p * L >= cfg.E && (cfg.kept == cfg.groups || (size % p == 0 && (lanes & (lanes - 1)) == 0));
+    route::Config c = cfg;
+    return p * L >= cfg.E && route::fit(c, p, L);
   };
-  if constexpr (L >= 16) {
-    if (cfg.kept < cfg.groups) {
-      if (fits(1)) return launch<T, 1, L>(a, cfg, s);
-      if (fits(3)) return launch<T, 3, L>(a, cfg, s);
-      if (fits(5)) return launch<T, 5, L>(a, cfg, s);
-      if (fits(6)) return launch<T, 6, L>(a, cfg, s);
-      if (fits(7)) return launch<T, 7, L>(a, cfg, s);
-    }
-  }
+  if constexpr (L >= 16)
+    if (grouped && fits(1)) return launch<T, 1, L>(a, cfg, s);
   if (fits(2)) return launch<T, 2, L>(a, cfg, s);
+  if constexpr (L >= 16)
+    if (grouped && fits(3)) return launch<T, 3, L>(a, cfg, s);
   if (fits(4)) return launch<T, 4, L>(a, cfg, s);
+  if constexpr (L >= 16) {
+    if (grouped && fits(5)) return launch<T, 5, L>(a, cfg, s);
+    if (grouped && fits(6)) return launch<T, 6, L>(a, cfg, s);
+    if (grouped && fits(7)) return launch<T, 7, L>(a, cfg, s);
+  }
   return launch<T, 8, L>(a, cfg, s);
 }
 
@@ -122,7 +125,8 @@ cudaError_t launch_typed(const B200MoeRouteArgs& a, const route::Config& cfg, cu
     if (cfg.E <= 32 && cfg.K <= 4) return launch_lanes<T, 4>(a, cfg, s);
     if (cfg.E <= 64 && cfg.K <= 8) return launch_lanes<T, 8>(a, cfg, s);
   }
-  if (cfg.E <= 128 && cfg.K <= 16) return launch_lanes<T, 16>(a, cfg, s);
+  route::Config half = cfg;
+  if (cfg.E <= 128 && cfg.K <= 16 && route::fit(half, 8, 16)) return launch_lanes<T, 16>(a, cfg, s);
   return launch_lanes<T, 32>(a, cfg, s);
 }
 
@@ -161,7 +165,8 @@ route::Config route_config(const B200MoeRouterConfig& c, int experts, int topk) 
   cfg.sigmoid = c.score == B200MOE_SCORE_SIGMOID;
   cfg.groups = c.groups;
   cfg.kept = c.kept_groups;
-  cfg.size = c.groups > 0 ? experts / c.groups : experts;   // 0 groups: a plan without a configured router
+  cfg.size = c.kept_groups < c.groups ? experts / c.groups : experts;
+  cfg.shift = -1;
   cfg.group_top2 = c.group_score == B200MOE_GROUP_TOP2;
   cfg.renormalize = c.renormalize != 0;
   cfg.bf16_weights = c.bf16_weights != 0;

@@ -83,13 +83,12 @@ router_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __r
   if (warp >= nt) return;
   // one warp per token: softmax, then K rounds of arg-max
   float* l = logits + warp * E;
-  if constexpr (kGeneral) {   // a configured router: route_row.cuh, eight consecutive experts per lane
+  if constexpr (kGeneral) {   // a configured router: route_row.cuh, eight experts per lane
     float row[8], b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) row[j] = lane * 8 + j < E ? l[lane * 8 + j] : -INFINITY;
-    route::load_bias<8>(cfg, bias, lane, b);
+    auto logit = [l](int e) { return l[e]; };
+    route::load_row<8, 32>(cfg, bias, lane, logit, row, b);
     const size_t o = static_cast<size_t>(t0 + warp) * K;
-    route::route_row<8, 32>(cfg, row, b, bias, lane, true, [l](int e) { return l[e]; },
+    route::route_row<8, 32>(cfg, row, b, bias, lane, true, logit,
                             route::Out{ids + o, rw + o, sizeof(IdT) == 8});
     return;
   }
@@ -146,9 +145,11 @@ cudaError_t launch_router(const B200MoePlan& p, cudaStream_t s) {
   auto* x = static_cast<const __nv_bfloat16*>(p.buf.x);
   auto* wr = static_cast<const __nv_bfloat16*>(p.buf.router_weight);
   auto* rw = static_cast<float*>(p.buf.routing_weights);
+  route::Config config = route_config(p);
+  route::fit(config, 8, 32);
   auto launch = [&](auto kernel, auto* ids) {
     kernel<<<grid, kRouterThreads, smem, s>>>(x, wr, ids, rw, sh.tokens, sh.experts, sh.hidden, sh.topk,
-                                              sh.router_bf16_weights, route_config(p),
+                                              sh.router_bf16_weights, config,
                                               static_cast<const float*>(p.buf.router_bias));
   };
   auto* ids64 = static_cast<long long*>(p.buf.ids);

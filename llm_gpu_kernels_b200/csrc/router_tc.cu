@@ -45,7 +45,7 @@ static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block too large");
 // kPerLane: experts per lane in the routing epilogue (ceil(E / 32) rounded up to 1, 2, 4 or 8): the top-k rounds
 // walk exactly the keys a lane holds.
 // kGeneral: a configured router (score function, bias, groups, ...): the row goes through route_row.cuh, for which a
-// lane holds kPerLane consecutive experts. The default router keeps the code below.
+// lane holds up to kPerLane experts. The default router keeps the code below.
 template <typename IdT, int kPerLane, bool kGeneral>
 __global__ void __launch_bounds__(kThreads, 1)
 router_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_wr,
@@ -177,9 +177,7 @@ router_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
           return sum_parts;
         };
         float l[kPerLane], b[kPerLane];
-#pragma unroll
-        for (int j = 0; j < kPerLane; ++j) l[j] = lane * kPerLane + j < E ? logit(lane * kPerLane + j) : -INFINITY;
-        route::load_bias<kPerLane>(cfg, bias, lane, b);
+        route::load_row<kPerLane, 32>(cfg, bias, lane, logit, l, b);
         const size_t o = static_cast<size_t>(t0 + r) * K;
         route::route_row<kPerLane, 32>(cfg, l, b, bias, lane, true, logit,
                                        route::Out{ids + o, rw + o, sizeof(IdT) == 8});
@@ -349,13 +347,16 @@ cudaError_t launch_router_typed(const B200MoePlan& p, cudaStream_t s, IdT* ids) 
   cfg.numAttrs = 2;
   int* status = static_cast<int*>(p.buf.scratch) + router_flag_index(p);  // folded into status by the dispatch
   auto* rw = static_cast<float*>(p.buf.routing_weights);
+  route::Config config = route_config(p);
   auto launch = [&](auto kernel) {
     return cudaLaunchKernelEx(&cfg, kernel, p.tm_x, p.tm_router_w, ids, rw, status, sh.tokens, sh.experts, sh.hidden,
-                              sh.topk, e_pad, p.router_stages, p.router_ksplit, sh.router_bf16_weights, route_config(p),
+                              sh.topk, e_pad, p.router_stages, p.router_ksplit, sh.router_bf16_weights, config,
                               static_cast<const float*>(p.buf.router_bias));
   };
   if (sh.use_router == 2) {
-    switch ((sh.experts + 31) / 32) {   // groups of a power-of-two number of lanes wherever their size allows it
+    int per_lane = (sh.experts + 31) / 32;
+    while (!route::fit(config, per_lane, 32) && per_lane < 8) ++per_lane;   // lanes for every group, where that is possible
+    switch (per_lane) {
       case 1: return launch(router_tc_kernel<IdT, 1, true>);
       case 2: return launch(router_tc_kernel<IdT, 2, true>);
       case 3: return launch(router_tc_kernel<IdT, 3, true>);

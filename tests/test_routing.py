@@ -179,6 +179,26 @@ def test_scores_closer_than_fp32(dev, score):
 
 
 @gpu
+@pytest.mark.parametrize("groups,size,topk,kept", [(4, 57, 8, 2), (3, 13, 4, 1), (8, 19, 8, 4), (2, 45, 16, 1), (3, 70, 6, 2),
+                                                   (5, 31, 7, 3), (7, 9, 5, 2), (3, 40, 12, 2), (16, 5, 4, 3), (2, 1, 1, 1),
+                                                   (32, 3, 2, 9), (3, 85, 32, 2), (6, 21, 10, 5), (2, 127, 9, 1)])
+@pytest.mark.parametrize("masked,biased,score,group_score,dtype", [
+    (0, True, "sigmoid", "top2", torch.float32), (0.5, False, "softmax", "top2", torch.bfloat16),
+    (0.2, True, "softmax", "max", torch.float16), (0, False, "sigmoid", "max", torch.float32)])
+def test_groups_of_any_size(dev, groups, size, topk, kept, masked, biased, score, group_score, dtype):
+    experts = groups * size
+    logits = make_logits(70, experts, dtype, 5 * experts + topk, dev, masked)
+    bias = (0.1 * torch.randn(experts, generator=torch.Generator().manual_seed(3))).to(dev) if biased else None
+    config = dict(score=score, groups=groups, kept_groups=kept, group_score=group_score)
+    p = prepare_routing(logits, topk, config=RouterConfig(**config), bias=bias)
+    agree(p.ids, p.routing_weights, logits, topk, bias, **config)
+    wide = torch.zeros(70, experts + 5, dtype=dtype, device=dev)   # rows at any address
+    wide[:, 3:3 + experts] = logits
+    q = prepare_routing(wide[:, 3:3 + experts], topk, config=RouterConfig(**config), bias=bias)
+    assert torch.equal(q.ids, p.ids) and torch.equal(q.routing_weights, p.routing_weights)
+
+
+@gpu
 @pytest.mark.parametrize("experts,topk,biased,config", [
     (256, 8, True, dict(score="sigmoid", groups=8, kept_groups=4, group_score="top2")),
     (256, 8, True, dict(score="sigmoid", groups=8, kept_groups=3)),
@@ -363,6 +383,9 @@ LAYERS = [
     (40, 40, 3, 67, 33, "generic", True, dict(score="sigmoid", groups=5, kept_groups=2, scale=0.5)),
     (9, 7, 2, 67, 33, "generic", False, dict(score="sigmoid")),
     (2500, 32, 2, 128, 64, "tcgen05", True, dict(groups=4, kept_groups=2)),
+    (64, 152, 8, 128, 64, "tcgen05", True, dict(score="sigmoid", groups=8, kept_groups=3, group_score="top2")),
+    (40, 225, 6, 128, 64, "tcgen05", True, dict(groups=3, kept_groups=2)),
+    (33, 39, 3, 67, 33, "generic", False, dict(groups=3, kept_groups=2)),
 ]
 
 
