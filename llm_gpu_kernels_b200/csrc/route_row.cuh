@@ -15,10 +15,9 @@
 // values closer than the error bound of that computation could be in the wrong order. Where two neighbours of the order
 // (or the groups at the border) are that close, one row in a thousand for random logits, the experts found (the two
 // largest of each group) are put in order by their c in FP64, one expert per lane (exact_order, exact_groups). That is
-// enough if the next expert is not close as well; otherwise, and in rows with fewer experts left than slots, the whole
-// row is routed in FP64 (route_exact). That pass takes 9 us for a row, most of it instruction fetches, and a single
-// late row shows in the call: with it alone 32768 rows x 256 experts took 41.5 us instead of 35.5, 4099 x 160 masked
-// 11.5 instead of 7.5.
+// enough if the next expert is not close as well; otherwise the whole row is routed in FP64 (route_exact). That pass
+// takes 9 us for a row, most of it instruction fetches, and a single late row shows in the call: with it alone 32768 rows
+// x 256 experts took 41.5 us instead of 35.5, 4099 x 160 masked 11.5 instead of 7.5.
 //
 // What bounds the common pass (route_fast) at many rows is the number of instructions per row, so it keeps the experts
 // of a lane as sorted 32-bit keys that hold the expert too: sorting eight is 19 compare-exchanges of two integer min /
@@ -26,7 +25,7 @@
 // the end by K lanes at once, from logits read again, so full-precision exp and division cost one instruction sequence
 // per row. 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups (5.4 us would be the HBM floor): 80 us with unsorted
 // keys and per-expert weights (1930 warp instructions per row), 47 us with sorted keys that leave ties and experts to
-// ballots (910), 35.5 us like this (930 instructions for a row that FP32 settles: 34.3 us if all did). Sixteen experts
+// ballots (910), 36 us like this (34.8 us if FP32 settled every row). Sixteen experts
 // per lane and two rows per warp need as many instructions per row (the warp-wide redux of 32 lanes becomes four
 // shuffles) and more registers: 73 us.
 #pragma once
@@ -371,6 +370,28 @@ __device__ __noinline__ uint32_t exact_order(const Config& cfg, const float* __r
   return mine;
 }
 
+// Lane n .. K-1: the (lane - n)-th lowest index that is not among the experts of lanes 0 .. n-1. Starting from that rank,
+// an index moves up by the chosen ones at or below it until it stays. (Left to route_exact, 8192 rows of 128 experts with
+// nine in ten masked took 36 us instead of 9.4.)
+template <int L>
+__device__ __noinline__ int fill_slot(int K, int lane, int n, int expert) {
+  int e = lane - n;
+  bool moved = true;
+#pragma unroll 1
+  while (moved) {
+    int below = 0;
+#pragma unroll 1
+    for (int i = 0; i < K; ++i) {
+      const int chosen = __shfl_sync(kAll, expert, i, L);
+      below += i < n && chosen <= e;
+    }
+    const int at = lane - n + below;
+    moved = __any_sync(kAll, lane >= n && lane < K && at != e);
+    e = at;
+  }
+  return e;
+}
+
 // Returns false when FP32 and a look at the candidates in FP64 cannot settle the row; otherwise slot `lane` < K of the
 // row is `expert` with weight `w`.
 // l[j]: logits of experts first + j (-inf: none), b[j]: biases.
@@ -540,10 +561,15 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
   const unsigned unfilled = sub_ballot<L>(empty);
   const bool nothing = (unfilled & 1u) != 0;   // a row whose mask leaves nothing: the lowest indices with weight 0
   const unsigned undecided = sub_ballot<L>(close);   // by every lane: not behind a condition that rows differ in
-  bool settled = nothing || (undecided == 0 && unfilled == 0);
+  bool settled = nothing || undecided == 0;
   *expert = nothing ? lane : static_cast<int>(255u - (won & 255u));
+  const bool partly = unfilled != 0 && !nothing;   // fewer experts left than slots
+  if (L == 32 ? partly : __any_sync(kAll, partly)) {
+    const int filler = fill_slot<L>(cfg.K, lane, cfg.K - __popc(unfilled), *expert);
+    if (empty) *expert = filler;
+  }
   float w = 0.0f;
-  if (lane < cfg.K && settled && !nothing) {
+  if (lane < cfg.K && settled && !empty) {
     const float x = load(*expert);
     w = cfg.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x == top ? 0.0f : x - top);
   }

@@ -179,6 +179,22 @@ def test_scores_closer_than_fp32(dev, score):
 
 
 @gpu
+@pytest.mark.parametrize("experts,topk,config", [
+    (128, 8, dict(groups=4, kept_groups=1)), (256, 32, dict(score="sigmoid")), (64, 8, {}), (16, 4, {}), (32, 32, {}),
+    (160, 6, dict(groups=8, kept_groups=2, group_score="top2", renormalize=False)), (57, 16, dict(score="sigmoid"))])
+@pytest.mark.parametrize("dtype,biased", [(torch.float32, True), (torch.bfloat16, False)])
+def test_rows_with_fewer_experts_than_slots(dev, experts, topk, config, dtype, biased):
+    g = torch.Generator().manual_seed(experts * topk)
+    logits = make_logits(200, experts, torch.float32, 17, torch.device("cpu"))
+    left = torch.randint(0, topk + 3, (200, 1), generator=g)      # experts that the mask leaves
+    logits[torch.rand(200, experts, generator=g).argsort(-1).argsort(-1) >= left] = -math.inf
+    logits = logits.to(dtype).to(dev)
+    bias = (0.1 * torch.randn(experts, generator=g)).to(dev) if biased else None
+    p = prepare_routing(logits, topk, config=RouterConfig(**config), bias=bias)
+    agree(p.ids, p.routing_weights, logits, topk, bias, **config)
+
+
+@gpu
 @pytest.mark.parametrize("groups,size,topk,kept", [(4, 57, 8, 2), (3, 13, 4, 1), (8, 19, 8, 4), (2, 45, 16, 1), (3, 70, 6, 2),
                                                    (5, 31, 7, 3), (7, 9, 5, 2), (3, 40, 12, 2), (16, 5, 4, 3), (2, 1, 1, 1),
                                                    (32, 3, 2, 9), (3, 85, 32, 2), (6, 21, 10, 5), (2, 127, 9, 1)])
