@@ -80,10 +80,11 @@ struct EpilogueWarp {
   alignas(16) float row_scale[kMaxTile];                 // of the tile it works on
   alignas(16) unsigned char transpose[16 * kPitch];      // 16 rows of its 32 channels
 };
-constexpr int epilogue_warps(bool split) { return split ? 0 : 8; }
-constexpr int ctrl_bytes(bool gate_up, bool split) {
-  return kCtrlBytes + epilogue_warps(split) *
-                          static_cast<int>(gate_up ? sizeof(EpilogueWarp<float>) : sizeof(EpilogueWarp<__half>));
+constexpr int kEpilogueWarps = 8;
+// Ctrl, and behind it what the epilogue needs: an EpilogueWarp each, or the row scales of a split tile.
+__host__ __device__ constexpr int ctrl_bytes(bool gate_up, bool split) {
+  return kCtrlBytes + (split ? kMaxTile * 4
+                             : kEpilogueWarps * static_cast<int>(gate_up ? sizeof(EpilogueWarp<float>) : sizeof(EpilogueWarp<__half>)));
 }
 
 // Rows 0 .. 15 (of which `rows` exist) of 32 channels from channel0: v[j] is row j of channel channel0 + lane. `dst` is
@@ -130,14 +131,14 @@ __device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr, uint32_t cta) {
 template <bool kGateUp, int kBoxes, bool kSplit, typename Out>
 __global__ void __launch_bounds__(kMaxThreads, 1)
 grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
-  constexpr int kEpilogueWarps = kSplit ? 4 : 8;
   static_assert(!kGateUp || kBoxes == 2, "gate and up are the two boxes");
   constexpr int kTileChannels = kGateUp ? kTileM : kBoxes * kTileM;
   constexpr uint32_t kWBytes = kBoxes * kBoxBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Ctrl* c = reinterpret_cast<Ctrl*>(smem_raw);
   const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t stage_off = ((raw_addr + ctrl_bytes(kGateUp, kSplit) + 1023u) & ~1023u) - raw_addr;
+  constexpr uint32_t kCtrl = ctrl_bytes(kGateUp, kSplit);
+  const uint32_t stage_off = ((raw_addr + kCtrl + 1023u) & ~1023u) - raw_addr;
   unsigned char* stages = smem_raw + stage_off;
   const int token_tile = g.token_tile, num_stages = g.stages;
   const uint32_t stage_bytes = kWBytes + static_cast<uint32_t>(token_tile) * kRowBytes;
@@ -191,6 +192,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
     item_step = total_items;
   }
   const bool any = first_item < total_items;
+  float* split_rows = reinterpret_cast<float*>(smem_raw + kCtrlBytes);   // the row scales of a split tile
   auto next_item = [&](int item) { return total_items - item > item_step ? item + item_step : total_items; };
 
   if (warp == 0) {
@@ -279,7 +281,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
         mbar_wait_plain(&c->drain[half], 0);
       }
     }
-  } else if (warp < kMmaWarpB || kEpilogueWarps == 8) {
+  } else {
     // ------------------------------------------------------------------ epilogue warps
     const int quarter = warp & 3;                      // the TMEM lane quarter this warp may read
     const int team = warp < kMmaWarpB ? 0 : 1;         // of the two warps of a quarter
@@ -287,6 +289,14 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
     int acc = 0;
     uint32_t acc_phase = 0;
     if (!kSplit) pdl_wait();   // row scales and output
+    if constexpr (kSplit) {
+      const int tile = blockIdx.x / ctas;   // also of a CTA without K blocks: it finishes rows
+      if (tile < total_items) {
+        const Tile t = decode_tile(&c->tables, tile, E, n_ct, token_tile);
+        pdl_wait();
+        for (int n = (team * 4 + quarter) * 32 + lane; n < t.rows; n += kEpilogueWarps * 32) split_rows[n] = g.row_scale[t.row0 + n];
+      }
+    }
     for (int item = first_item; item < total_items; item = next_item(item)) {
       const Tile t = decode_tile(&c->tables, item, E, n_ct, token_tile);
       const int channel = t.ct * kTileChannels + quarter * 32 + lane;      // of the first box
@@ -307,7 +317,7 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       if (kSplit) {
         // partial sums [box][row][128], for the cluster, into the drained stages
         int* part = reinterpret_cast<int*>(stages) + quarter * 32 + lane;
-        for (int n0 = 0; n0 < t.n_eff; n0 += 16) {
+        for (int n0 = team * 16; n0 < t.n_eff; n0 += 32) {
           uint32_t a[16], b[16];
           tmem_ld16(taddr + n0, a);
           tmem_ld16(taddr + token_tile + n0, b);
@@ -364,50 +374,60 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
     // ------------------------------------------------------------------ the cluster's partial sums -> output
     __syncwarp();
     cluster_barrier();   // every CTA's partial sums are in its shared memory
-    pdl_wait();          // row scales and output
+    pdl_wait();          // output
     const int tile = blockIdx.x / ctas;
     if (tile < total_items && !*reinterpret_cast<volatile int*>(&c->abort)) {
       const Tile t = decode_tile(&c->tables, tile, E, n_ct, token_tile);
       const int per = (num_kb + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
       const int active = (num_kb + per - 1) / per;   // CTAs that had K blocks
       const uint32_t base = smem_u32(stages) + static_cast<uint32_t>(lane) * 16u;
-      const float* scales = g.w_scale + static_cast<size_t>(t.expert) * g.w_rows;
       Out* dst = static_cast<Out*>(g.out) + static_cast<size_t>(t.row0) * g.n_out;
-      // a unit is one row of one box (gate/up: of both); units go round the CTAs, then the warps
-      const int units = (kBoxes == 2 && !kGateUp ? 2 : 1) * t.rows;
-      for (int u = static_cast<int>(cta) + static_cast<int>(ctas) * warp; u < units;
-           u += static_cast<int>(ctas) * kMaxThreads / 32) {
-        const int n = u % t.rows, box = u / t.rows;
-        const int channel = t.ct * kTileChannels + box * kTileM + lane * 4;
-        const float row_scale = g.row_scale[t.row0 + n];
-        int sum[4] = {}, sum_up[4] = {};
-        int4 v[kMaxSplit], w[kGateUp ? kMaxSplit : 1];   // all loads first: one round trip
+      // the scales of this lane's four channels, of gate and up or of both boxes
+      const float* scales = g.w_scale + static_cast<size_t>(t.expert) * g.w_rows;
+      float split_scale[kBoxes][4] = {};
 #pragma unroll
-        for (int i = 0; i < kMaxSplit; ++i) {
-          if (i < active) {
-            v[i] = ld_cluster_int4(base + static_cast<uint32_t>((box * token_tile + n) * kTileM * 4), i);
-            if constexpr (kGateUp) w[i] = ld_cluster_int4(base + static_cast<uint32_t>((token_tile + n) * kTileM * 4), i);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kMaxSplit; ++i) {
-          if (i < active) {
-            sum[0] += v[i].x; sum[1] += v[i].y; sum[2] += v[i].z; sum[3] += v[i].w;
-            if constexpr (kGateUp) {
-              sum_up[0] += w[i].x; sum_up[1] += w[i].y; sum_up[2] += w[i].z; sum_up[3] += w[i].w;
-            }
-          }
-        }
-        Out* row = dst + static_cast<size_t>(n) * g.n_out + channel;
+      for (int b = 0; b < kBoxes; ++b)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (channel + j < g.n_out) {
-            const float v = scaled(static_cast<uint32_t>(sum[j]), row_scale * scales[channel + j]);
-            if constexpr (kGateUp)
-              store_out(row + j, swiglu(v, scaled(static_cast<uint32_t>(sum_up[j]), row_scale * scales[g.n_out + channel + j])));
-            else
-              store_out(row + j, v);
-          }
+          const int channel = t.ct * kTileChannels + (kGateUp ? 0 : b * kTileM) + lane * 4 + j;
+          if (channel < g.n_out) split_scale[b][j] = scales[kGateUp ? b * g.n_out + channel : channel];
+        }
+      // Each CTA finishes every ctas-th row, a warp two vectors of 4 channels x 32 lanes at a time: gate and up of a row,
+      // its two boxes, or with one box two rows. All loads of the two come first: one round trip through the cluster.
+      constexpr int kRows = kBoxes == 2 ? 1 : 2;
+      const int stride = static_cast<int>(ctas) * kMaxThreads / 32;
+      for (int n = static_cast<int>(cta) + static_cast<int>(ctas) * warp; n < t.rows; n += kRows * stride) {
+        int4 v[2][kMaxSplit];
+        const int vectors = kRows == 2 && n + stride >= t.rows ? 1 : 2;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int at = kRows == 2 ? n + b * stride : b * token_tile + n;
+#pragma unroll
+          for (int i = 0; i < kMaxSplit; ++i)
+            if (i < active && b < vectors) v[b][i] = ld_cluster_int4(base + static_cast<uint32_t>(at * kTileM * 4), i);
+        }
+        float y[2][4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          int sum[4] = {};
+#pragma unroll
+          for (int i = 0; i < kMaxSplit; ++i)
+            if (i < active) {
+              sum[0] += v[b][i].x; sum[1] += v[b][i].y; sum[2] += v[b][i].z; sum[3] += v[b][i].w;
+            }
+          const float row_scale = split_rows[kRows == 2 ? min(n + b * stride, t.rows - 1) : n];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[b][j] = scaled(static_cast<uint32_t>(sum[j]), row_scale * split_scale[kRows == 2 ? 0 : b][j]);
+        }
+#pragma unroll
+        for (int b = 0; b < (kGateUp ? 1 : 2); ++b) {
+          const int row = kRows == 2 ? n + b * stride : n;
+          const int channel = t.ct * kTileChannels + (kRows == 2 ? 0 : b * kTileM) + lane * 4;
+          if (row >= t.rows) break;
+          Out* to = dst + static_cast<size_t>(row) * g.n_out + channel;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (channel + j < g.n_out) store_out(to + j, kGateUp ? swiglu(y[0][j], y[1][j]) : y[b][j]);
         }
       }
     }
@@ -482,7 +502,9 @@ double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxe
   if (block < 210.0) block = 210.0;
   const double rows = static_cast<double>(token_tile) * boxes;
   if (split > 1) {
-    if (tiles * split > sms || blocks < 2 * split) return -1.0;
+    // All clusters have to be resident at once: pairs take every SM, clusters of 4 leave out two SMs of a GPC, of 8 there
+    // are two in most GPCs but not in all (128 rows x 8192 x 1024: 16 clusters of 8 18.5 us, half as many CTAs 13.6).
+    if (tiles * split > (split == 8 ? sms * 2 / 3 : split == 4 ? sms * 7 / 8 : sms) || blocks < 2 * split) return -1.0;
     return (blocks + split - 1) / split * block + 3200.0 + 38.0 * rows;
   }
   const double rounds = static_cast<double>((tiles + sms - 1) / sms);
