@@ -487,7 +487,7 @@ int i8_stages(bool gate_up, int boxes, int token_tile, int split, int* smem_byte
 // What decides between tile shapes, with figures fitted to 33 timings of 9 to 2048 rows (k 1999 to 4096, n 1536 to 5003;
 // all but four within 12 %). A stage takes the longest of its bytes at 50 bytes per cycle out of L2, its MMAs (half a
 // cycle per row and K step of 32) and 210 cycles of hand-over; a tile that is not followed by another on its SM shows
-// its epilogue, 36 cycles per row and box; adding up a split tile takes 3200 cycles and 38 per row and box. Above 512
+// its epilogue, 36 cycles per row and box; adding up a split tile takes 3200 cycles and 26 per row and box. Above 512
 // columns of accumulators there is only one set and every epilogue shows, at 30 cycles per row and box with eight warps:
 // 128 x 2 boxes is faster while K is short (8192 x 1024 x 4096: 54 and 66 us), 256 x 2 once K is long, where the power
 // limit decides and a third less goes through L2 (8192 x 4096 x 14336, back to back for seconds: 442 and 421 us).
@@ -505,7 +505,7 @@ double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxe
     // All clusters have to be resident at once: pairs take every SM, clusters of 4 leave out two SMs of a GPC, of 8 there
     // are two in most GPCs but not in all (128 rows x 8192 x 1024: 16 clusters of 8 18.5 us, half as many CTAs 13.6).
     if (tiles * split > (split == 8 ? sms * 2 / 3 : split == 4 ? sms * 7 / 8 : sms) || blocks < 2 * split) return -1.0;
-    return (blocks + split - 1) / split * block + 3200.0 + 38.0 * rows;
+    return (blocks + split - 1) / split * block + 3200.0 + 26.0 * rows;
   }
   const double rounds = static_cast<double>((tiles + sms - 1) / sms);
   if (rounds > 1 && 4 * token_tile > 512) return rounds * (blocks * block + 30.0 * rows);
