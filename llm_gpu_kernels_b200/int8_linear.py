@@ -34,6 +34,7 @@ class PreparedInt8Linear:
     _plan: object = field(default=None, repr=False)
     _call: object = field(default=None, repr=False)
     _device: int = field(default=0, repr=False)
+    _written: tuple = field(default=(), repr=False)
 
     def run(self):
         """One product on the current stream; returns ``output``."""
@@ -41,7 +42,7 @@ class PreparedInt8Linear:
             _ops.int8_linear(self._plan.value, self.x, self.weight.storage, self.weight.scales, self.output, self.x_q,
                              self.x_scale, self.status)
         elif self.x.shape[0]:
-            _native.launch(self._call, self._plan, self._device, (self.output, self.x_q, self.x_scale, self.status))
+            _native.launch(self._call, self._plan, self._device, self._written)
         return self.output
 
     def check(self):
@@ -99,6 +100,7 @@ def prepare_int8_linear(x, weight, *, output=None):
         lib.b200moe_linear_destroy(handle)
         raise
     prepared._plan, prepared._call, prepared._device = handle, lib.b200moe_linear_forward, device.index
+    prepared._written = (output, prepared.x_q, prepared.x_scale, prepared.status)
     _ops.register_linear(prepared)
     prepared.run()
     return prepared

@@ -90,6 +90,7 @@ class PreparedRouting:
     _args: object = field(default=None, repr=False)
     _call: object = field(default=None, repr=False)
     _device: int = field(default=0, repr=False)
+    _written: tuple = field(default=(), repr=False)
 
     def run(self):
         """Routes every row on the current stream; returns (ids, routing_weights)."""
@@ -98,7 +99,7 @@ class PreparedRouting:
             _ops.route(self.logits, self.bias, self.ids, self.routing_weights, SCORES[c.score], c.groups, c.kept,
                        GROUP_SCORES[c.group_score], c.renormalize, float(c.scale))
         elif self.logits.shape[0]:
-            _native.launch(self._call, self._args, self._device, (self.ids, self.routing_weights))
+            _native.launch(self._call, self._args, self._device, self._written)
         return self.ids, self.routing_weights
 
 
@@ -138,6 +139,6 @@ def prepare_routing(logits, topk, *, config=RouterConfig(), bias=None, ids=None,
         config=config.native(), logits=logits.data_ptr(), bias=bias.data_ptr() if bias is not None else None,
         ids=ids.data_ptr(), weights=routing_weights.data_ptr())
     prepared = PreparedRouting(logits, topk, config, bias, ids, routing_weights, args, _native.load().b200moe_route,
-                               device.index)
+                               device.index, (ids, routing_weights))
     prepared.run()
     return prepared
