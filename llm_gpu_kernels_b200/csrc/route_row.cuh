@@ -49,6 +49,8 @@ struct Config {
 };
 
 constexpr int kMaxGroups = 32;
+constexpr float kFarBelow = -1e30f;   // c at or below it has no place of its own among a row's FP32 keys
+constexpr float kSteps = 16777208.0f; // places between the smallest and the largest c: with 3 for rounding below 2^24 - 2
 
 // Lays a row out over L lanes of P experts: a group has a power of two of whole lanes to itself, the last of them filled
 // up with nothing, so that its values meet in a few shuffles. False (shift -1): the groups need more lanes than there
@@ -399,8 +401,9 @@ __device__ __noinline__ int fill_slot(int K, int lane, int n, int expert) {
 // Keys are (q << 8) | (255 - expert): the larger key has the larger q, or the lower index at equal q, so every key is
 // different, the winner of a round names its expert and no tie needs a second look. q has 24 bits and is at least 1
 // (key 0: not a candidate). Logits of 16 bits without a bias give their leading 24 bits, which are exact. Everything
-// else gives its place between the smallest and the largest c of the row (values below -1e30 count as the smallest):
-// q = 1 + (c - base) * scale, monotonic in c and off by less than 2 from rounding.
+// else gives its place between the smallest and the largest c of the row: q = 2 + (c - base) * scale, monotonic in c and
+// off by less than 2 from rounding. Values of -1e30 and less, the lowest finite ones that programs mask experts with,
+// stay out of that range and are all q = 1: behind every other expert, in an order that only FP64 knows.
 template <int P, int L, typename Load>
 __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], const float (&b)[P], int lane, int first,
                                            const float* __restrict__ bias, Load load, int* expert, float* weight) {
@@ -444,9 +447,10 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
     }
   }
   uint32_t key[P];
-  float base = 0.0f, step = 0.0f;    // c = base + (q - 1) * step, about
+  float base = 0.0f, step = 0.0f;    // c = base + (q - 2) * step, about
   uint32_t unsure = 0;               // two q this close or closer may be in the wrong order
   bool close = false;
+  bool vague = false;                // the keys do not tell what groups are worth
   if (exact) {
 #pragma unroll
     for (int j = 0; j < P; ++j)   // + 0: zeros of both signs tie
@@ -455,7 +459,7 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
     float low = INFINITY, high = none;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      low = fminf(low, c[j] > -1e30f ? c[j] : INFINITY);
+      low = fminf(low, c[j] > kFarBelow ? c[j] : INFINITY);
       high = fmaxf(high, c[j]);
     }
     if (biased) high = K::value(sub_max<L>(K::of(high)));
@@ -464,12 +468,13 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
     low = fminf(low, high);
     const float range = high - low;
     // a row of one value, or with an infinity: every q is the same, which settles nothing
-    const float scale = range > 1e-30f && range < INFINITY ? 16777212.0f / range : 0.0f;
+    const float scale = range > 1e-30f && range < INFINITY ? kSteps / range : 0.0f;
     base = low;
-    step = scale > 0.0f ? range / 16777212.0f : 0.0f;
+    step = scale > 0.0f ? range / kSteps : 0.0f;
+    const float least = scale > 0.0f ? -1.0f : 0.0f;   // for c below `low`
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      const float q = fmaxf(0.0f, (c[j] - low) * scale) + 1.0f;   // NaN (infinities) -> 1
+      const float q = fmaxf(least, (c[j] - low) * scale) + 2.0f;   // NaN (infinities): scale is 0, q 2
       key[j] = c[j] > none ? __float2uint_rn(q) << 8 | (255u - (first + j)) : 0u;
     }
     // The error of c: __expf is within 2^-22 + |x| 2^-23, which moves a sigmoid by a quarter of that and a softmax score
@@ -479,6 +484,9 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       const float widest = fmaxf(fabsf(low), fabsf(high));
       unsure = static_cast<uint32_t>(fminf(2.0f * ((cfg.sigmoid ? 4e-7f : 1.5e-6f * unit) + 6e-8f * widest) * scale + 5.0f, 16777215.0f));
     }
+    // Scores are compared by logits a step or two off, so a step has to be small. A sum with a c far below is taken for
+    // less than any two other c, which holds while these are not of its size.
+    vague = scale == 0.0f || (cfg.group_top2 && (biased ? !(2.0f * low > high + kFarBelow) : step > 0.1f));
   }
   sort_keys<P>(key);
   if (grouped) {
@@ -490,15 +498,22 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       a = max(a, oa);
     }
     auto value_of = [&](uint32_t k) {
-      return exact ? K::value(k & ~255u) : base + static_cast<float>((k >> 8) - 1u) * step;
+      return exact ? K::value(k & ~255u) : base + static_cast<float>(static_cast<int>(k >> 8) - 2) * step;
     };
+    auto far_below = [](uint32_t k) { return k < 512u; };   // q = 1; exact keys are larger
     const bool by_score = cfg.group_top2 && !biased;
+    // Far below: the score is 0, and so it is in FP64, at more than 1e22 under the largest logit (or 1e30 under 0). A c
+    // there is unknown, and so is a sum with it: such groups tie with each other and come before those that have nobody.
+    constexpr float kUnknown = -3e38f;
     float value = none;
     if (a) {
-      value = value_of(a);
-      if (cfg.group_top2) {
-        if (by_score) value = score(value);
-        if (second) value += by_score ? score(value_of(second)) : value_of(second);
+      if (by_score) {
+        value = far_below(a) ? 0.0f : score(value_of(a));
+        if (second) value += far_below(second) ? 0.0f : score(value_of(second));
+      } else if (cfg.group_top2 && second) {
+        value = far_below(second) ? kUnknown : value_of(a) + value_of(second);
+      } else {
+        value = far_below(a) ? kUnknown : value_of(a);
       }
     }
     const int leader = lane & ~(lanes - 1);   // of this lane's group
@@ -515,7 +530,7 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       const float border = K::value(last), next = K::value(sub_max<L>(group_key));
       // two values of two c each (or scores, whose logits are off by `step`)
       const float far = by_score ? 4.0f * (2e-6f * unit + step) : 2.0f * step * static_cast<float>(unsure + 2u) + 2.4e-7f * fabsf(border);
-      close = border - next <= far;   // infinities compare false
+      close = vague || border - next <= far;   // infinities compare false
       if (__any_sync(kAll, close)) {
         // In FP64 from the two largest of each group. They have to be certain: no third one close to the second.
         int near = 0;

@@ -536,3 +536,57 @@ def test_expert_side_has_no_router(monkeypatch):
     token, expert = calls
     assert all(token[name] is value for name, value in how.items())
     assert not any(name in expert and expert[name] is not None for name in how)
+
+
+# ---- finite masks: the lowest value of a type and others that stand for "not this one"
+FINITE_MASKS = [torch.finfo(torch.float32).min, -1e31, -1.0000001e30, -1e30, -1e29, -1e9]
+MASKED_GROUPS = [
+    # groups, size, kept, topk
+    (2, 4, 1, 2), (8, 4, 3, 6), (8, 32, 4, 8), (4, 57, 2, 8), (3, 13, 1, 4), (16, 5, 4, 3), (32, 2, 9, 4), (3, 70, 2, 6)]
+
+
+def few_left(rows, groups, size, mask, g):
+    """[rows, groups * size] factors of a mask: each group keeps none, one, two or all of its experts."""
+    left = torch.tensor([0, 1, 1, 2, size])[torch.randint(0, 5, (rows, groups, 1), generator=g)]
+    out = torch.rand(rows, groups, size, generator=g).argsort(-1).argsort(-1) >= left
+    return out.view(rows, groups * size)
+
+
+@gpu
+@pytest.mark.parametrize("groups,size,kept,topk", MASKED_GROUPS)
+@pytest.mark.parametrize("mask", FINITE_MASKS)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_finite_masks_in_groups(dev, groups, size, kept, topk, mask, score):
+    """A masked expert counts with the value it has, not with that of the worst one that is left."""
+    g = torch.Generator().manual_seed(groups * size + kept)
+    experts = groups * size
+    logits = make_logits(90, experts, torch.float32, experts + kept, torch.device("cpu"))
+    out = few_left(90, groups, size, mask, g)
+    logits[:60][out[:60]] = mask
+    logits[50:60] = torch.where(out[50:60], mask, 0.1)            # all that is left is alike
+    logits[40:50] = torch.where(out[40:50], 2 * torch.tensor(mask), logits[40:50])   # -inf for the lowest value
+    logits = logits.to(dev)
+    bias = 0.1 * torch.randn(experts, generator=g)
+    for b in (None, bias, torch.where(out[0], mask, bias), torch.where(out[1], mask, bias)):
+        b = b.to(dev) if b is not None else None
+        for group_score in ("top2", "max"):
+            config = dict(score=score, groups=groups, kept_groups=kept, group_score=group_score)
+            p = prepare_routing(logits, topk, config=RouterConfig(**config), bias=b)
+            agree(p.ids, p.routing_weights, logits, topk, b, **config)
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("group_score", ["top2", "max"])
+def test_values_as_low_as_masks_in_groups(dev, score, group_score):
+    """Ordinary values among which some lie near -1e30: two of them add up to less than one and a mask."""
+    g = torch.Generator().manual_seed(19)
+    values = torch.tensor([0.5, -9e29, -6e29, -4e29, -1e29, -1e30, -1.2e30, -1.9e30, -3e38, -1e38, 1e30, 2.5])
+    logits = values[torch.randint(0, 12, (400, 32), generator=g)]
+    bias = values[torch.randint(0, 11, (32,), generator=g)]
+    for groups, kept in ((8, 3), (16, 5), (4, 2)):
+        config = dict(score=score, groups=groups, kept_groups=kept, group_score=group_score)
+        for l, b in ((logits, None), (logits, bias), (torch.randn(400, 32, generator=g), bias)):
+            l, b = l.to(dev), b.to(dev) if b is not None else None
+            p = prepare_routing(l, 4, config=RouterConfig(**config), bias=b)
+            agree(p.ids, p.routing_weights, l, 4, b, **config)
