@@ -156,9 +156,9 @@ class PreparedMoE:
         self._stage(4)
 
     def run(self):
-        """One forward on the current stream (``b200moe_forward``). While ``torch.compile`` or another tracer records,
-        the call goes through the registered PyTorch operator ``torch.ops.b200moe.forward``, which tells the tracer
-        what it writes."""
+        """One forward on the current stream (``b200moe_forward``). While ``torch.compile`` or another recorder of
+        operators (``_native.tracing``) is at work, the call goes through the registered PyTorch operator
+        ``torch.ops.b200moe.forward``, which tells it what is written."""
         if self.x.shape[0] == 0:
             return self.output
         if self._op_args is None:
