@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define B200MOE_ABI_VERSION 5
+#define B200MOE_ABI_VERSION 6
 
 /* error codes */
 #define B200MOE_OK 0
@@ -135,7 +135,7 @@ typedef struct {
   size_t ranks;         /* [R] int32 */
   size_t grouped_input; /* [R,H] bf16 */
   size_t activated;     /* [R,I] bf16; INT8 plans: [R,I] float32, quantised into activated_q */
-  size_t down_output;   /* [R,H] bf16 */
+  size_t down_output;   /* [R,H] bf16; INT8 plans: [R,H] float32 */
   size_t status;        /* [1] int32 */
   size_t scratch;       /* dispatch partial histograms, router flag, tile counter and per-expert completion
                            counters of the chained GEMM kernels */

@@ -14,7 +14,7 @@ from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libb200moe.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 STATUS_BAD_ID = 1
 STATUS_BAD_WEIGHT = 2

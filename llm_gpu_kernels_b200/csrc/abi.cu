@@ -189,7 +189,7 @@ int bind_int8(B200MoePlan& p) {
           }
         }
     int smem = 0;
-    g.stages = i8_stages(first_box == 2, g.boxes, p.token_tile, g.split, &smem);
+    g.stages = i8_stages(4, g.boxes, p.token_tile, g.split, &smem);
     const long long items = most * ((g.n_out + (first_box == 2 ? 128 : 128 * g.boxes) - 1) / (first_box == 2 ? 128 : 128 * g.boxes));
     g.grid = static_cast<int>(g.split > 1 ? items * g.split : items < p.num_sms ? items : p.num_sms);
   };
@@ -224,7 +224,7 @@ int launch_int8_small(const B200MoePlan& p, bool gate_up, cudaStream_t s) {
   a.x = gate_up ? b.x : b.activated;
   a.weight = static_cast<const int8_t*>(gate_up ? b.gate_up : b.down);
   a.w_scale = static_cast<const float*>(gate_up ? b.gate_up_scales : b.down_scales);
-  a.y = gate_up ? b.activated : b.down_output;
+  a.y = static_cast<float*>(gate_up ? b.activated : b.down_output);
   a.q = static_cast<int8_t*>(gate_up ? b.x_q : b.activated_q);
   a.q_scale = static_cast<float*>(gate_up ? b.x_scale : b.activated_scale);
   a.ids = b.ids;
@@ -248,7 +248,7 @@ int launch_int8_down(const B200MoePlan& p, cudaStream_t s) {
   q.q = static_cast<int8_t*>(p.buf.activated_q);
   q.scale = static_cast<float*>(p.buf.activated_scale);
   cudaError_t e = launch_quantize_rows(q, s);
-  if (e == cudaSuccess) e = launch_i8_product(p.i8_down, B200MOE_BF16, s);
+  if (e == cudaSuccess) e = launch_i8_product(p.i8_down, B200MOE_FP32, s);
   return check_cuda(e, "down launch");
 }
 
@@ -444,7 +444,7 @@ int b200moe_plan_create(const B200MoeShape* shape, B200MoePlan** out) {
   w.ranks = R * 4;
   w.grouped_input = R * H * 2;
   w.activated = s.route_only ? 0 : R * I * (is_int8(s) ? 4 : 2);
-  w.down_output = R * H * 2;
+  w.down_output = R * H * (is_int8(s) ? 4 : 2);
   w.status = 4;
   w.scratch = align256((static_cast<size_t>(p->partitions) * E + blocks + 2 + E) * 4);
   w.source_rows = p->gather ? R * 4 : 0;

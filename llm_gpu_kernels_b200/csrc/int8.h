@@ -40,7 +40,7 @@ struct LayerSmall {
   const void* x;             // gate/up: BF16 rows of the tokens; down: FP32 rows in grouped order
   const int8_t* weight;
   const float* w_scale;
-  void* y;                   // gate/up: FP32 [routes, n_out]; down: BF16; both in grouped order
+  float* y;                  // [routes, n_out] in grouped order
   int8_t* q;                 // the quantised rows and their scales, for whoever reads the workspace
   float* q_scale;
   const void* ids;
@@ -67,7 +67,7 @@ struct I8Gemm {
   int split;                   // CTAs of a cluster that share a tile's K; 1: persistent CTAs, a tile each
   int grid;
 };
-int i8_stages(bool gate_up, int boxes, int token_tile, int split, int* smem_bytes);
+int i8_stages(int out_bytes, int boxes, int token_tile, int split, int* smem_bytes);   // out_bytes: of an output value
 // Cycles that a product of `row_tiles` tiles of `token_tile` rows with n_out channels and k values would take in the
 // given form, or -1 where the form does not exist. See grouped_gemm_i8.cu.
 double i8_cycles(long long row_tiles, int n_out, int k, int token_tile, int boxes, int split, int sms);

@@ -107,11 +107,10 @@ layer_small_kernel(const LayerSmall a) {
       if (lane == 0) {
         const float gate = static_cast<float>(s0) * (scale.scale * w_scale[n]);
         const float up = static_cast<float>(s1) * (scale.scale * w_scale[n + second]);
-        static_cast<float*>(a.y)[out] = (gate / (1.0f + __expf(-gate))) * up;
+        a.y[out] = (gate / (1.0f + __expf(-gate))) * up;
       }
     } else if (lane < 2 && n + lane < a.n_out) {
-      static_cast<__nv_bfloat16*>(a.y)[out + lane] =
-          __float2bfloat16_rn(static_cast<float>(lane ? s1 : s0) * (scale.scale * w_scale[n + lane]));
+      a.y[out + lane] = static_cast<float>(lane ? s1 : s0) * (scale.scale * w_scale[n + lane]);
     }
   }
 }

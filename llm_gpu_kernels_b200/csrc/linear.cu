@@ -158,7 +158,7 @@ int b200moe_linear_bind(B200MoeLinear* p, const B200MoeLinearBuffers* b) {
   g.boxes = p->boxes;
   g.split = p->split;
   int smem = 0;
-  g.stages = i8_stages(false, g.boxes, g.token_tile, g.split, &smem);
+  g.stages = i8_stages(2, g.boxes, g.token_tile, g.split, &smem);
   g.stream_weights = s.tokens <= p->token_tile;
   const long long items = static_cast<long long>((s.tokens + p->token_tile - 1) / p->token_tile) *
                           ((s.n + 128 * p->boxes - 1) / (128 * p->boxes));

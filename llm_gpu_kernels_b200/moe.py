@@ -322,7 +322,8 @@ def _prepare(x, gate_up, down, ids, routing_weights, *, router_weight=None, sche
             int32((e,)), int32((e,)), int32((e,)), int32((e + 1,)), int32((r,)),
             bf16((0 if sizes.gathers or int8 else r, h)), bf16((0, 2 * intermediate)),
             torch.empty((0 if route_only_experts is not None else r, intermediate), device=device,
-                        dtype=torch.float32 if int8 else torch.bfloat16), bf16((r, h)),
+                        dtype=torch.float32 if int8 else torch.bfloat16),
+            torch.empty((r, h), device=device, dtype=torch.float32 if int8 else torch.bfloat16),
             int32((1,)), config,
             ranks=int32((r,)), scratch=int32((max(1, sizes.scratch // 4),)), router_weight=router_weight,
             router=router, router_bias=router_bias, schedule=_native.SCHEDULE_NAMES[sizes.schedule], token_tile=sizes.token_tile,

@@ -7,8 +7,9 @@ moe_w4_cuda.py:85-164).
     output          = sum over a token's routes of routing weight * (q(a) . Wd^T) * row scale * channel scale
 
 Half the weight bytes of BF16 experts and twice their tensor rate. Life cycle, dispatch, combine, router and
-attributes are those of ``prepare_moe``; ``activated`` is FP32 here, and ``x_q`` / ``x_scale`` / ``activated_q`` /
-``activated_scale`` are the quantised rows, in grouped order. Any H and I up to 131072 work (rows are padded to 16 bytes).
+attributes are those of ``prepare_moe``; ``activated`` and ``down_output`` are FP32 here, so that BF16 comes with the
+result only, and ``x_q`` / ``x_scale`` / ``activated_q`` / ``activated_scale`` are the quantised rows, in grouped order. Any
+H and I up to 131072 work (rows are padded to 16 bytes).
 A token whose row holds an infinity or a NaN gives NaN in that row only.
 """
 from .int8_weights import Int8Weight

@@ -581,3 +581,31 @@ def test_expert_parallelism_refuses():
 def test_quantize_int8_refuses_empty(shape):
     with pytest.raises(ValueError):
         quantize_int8(torch.zeros(shape))
+
+
+# ---- precision and length of the layer
+@gpu
+@pytest.mark.parametrize("t,e,k,h,i,tile", [(1, 8, 8, 256, 128, 0), (1, 8, 2, 67, 33, 16), (2, 4, 2, 264, 70, 0), (40, 8, 2, 256, 128, 0),
+                                            (33, 5, 3, 200, 130, 0), (300, 4, 4, 1030, 72, 0), (900, 2, 2, 384, 256, 256)])
+def test_rows_are_rounded_once(dev, t, e, k, h, i, tile):
+    """Down rows and their weighted sum stay in FP32; BF16 comes with the result. y: two scales and the sum, four
+    roundings of 2^-24; the combine: K products and additions."""
+    x, gate_up, down, ids, rw = layer_inputs(t, e, k, h, i, "random", dev, seed=4)
+    p = prepare_int8_moe(x, gate_up, down, ids, rw, token_tile=tile)
+    base = p.base
+    assert base.down_output.dtype == torch.float32
+    mapping = base.mapping.cpu().long().view(t, k)
+    a = base.activated_q[:, :i].cpu().double()[mapping]            # [t, k, i]
+    dvalues, dscales = down.values.cpu().double(), down.scales.cpu().double()
+    ids = ids.cpu().long()
+    y = torch.empty(t, k, h, dtype=torch.float64)
+    for expert in range(e):
+        at = ids == expert
+        y[at] = (a[at] @ dvalues[expert].T) * dscales[expert]
+    y *= base.activated_scale.cpu().double()[mapping][..., None]
+    got = base.down_output.cpu().double()[mapping]
+    assert not ((got - y).abs() > 2.0 ** -21 * y.abs()).any()
+    terms = y * rw.cpu().double()[..., None]
+    want, out = terms.sum(1), base.output.cpu().double()
+    limit = HALF[torch.bfloat16] * want.abs() + (2.0 ** -21 + (k + 1) * 2.0 ** -24) * terms.abs().sum(1)
+    assert not ((out - want).abs() > limit).any()
