@@ -38,8 +38,10 @@
 // short burst, 2.86 POP/s, tensor pipe busy 72 % of its cycles; 404 us for seconds under the power limit).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "gemm_tile.cuh"
 #include "int8.h"
+#include "int8_rows.cuh"
 #include "pdl.cuh"
 #include "plan.h"
 #include "sm100_ptx.cuh"
@@ -115,7 +117,33 @@ __device__ __forceinline__ void store_rows(Out* dst, const float (&v)[16], int r
   }
 }
 
-__device__ __forceinline__ float scaled(uint32_t sum, float scale) { return static_cast<float>(static_cast<int>(sum)) * scale; }
+// kFar: some products of two scales of the tile may be out of range; see rows8::scaled.
+template <bool kFar>
+__device__ __forceinline__ float scaled(uint32_t sum, float row, float channel) {
+  return kFar ? rows8::scaled(static_cast<int>(sum), row, channel) : static_cast<float>(static_cast<int>(sum)) * (row * channel);
+}
+// Four channels of a row; out of line, for the same reason.
+__device__ __noinline__ float4 scaled_far4(int4 sum, float row, float4 channel) {
+  return make_float4(rows8::scaled(sum.x, row, channel.x), rows8::scaled(sum.y, row, channel.y),
+                     rows8::scaled(sum.z, row, channel.z), rows8::scaled(sum.w, row, channel.w));
+}
+// The smallest and the largest finite scale above 0 of some rows, as bits.
+struct RowScales {
+  uint32_t least = 0x7f800000u, most = 0u;
+  __device__ __forceinline__ void add(float s) {
+    if (s > 0.0f && s < INFINITY) {
+      least = min(least, __float_as_uint(s));
+      most = max(most, __float_as_uint(s));
+    }
+  }
+  __device__ __forceinline__ void join() {   // those of the warp's lanes
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+  }
+  __device__ __forceinline__ bool far(float channel) const {
+    return channel != 0.0f && most != 0u && !(rows8::in_range(__uint_as_float(least) * channel) && rows8::in_range(__uint_as_float(most) * channel));
+  }
+};
 __device__ __forceinline__ float swiglu(float gate, float up) { return (gate / (1.0f + __expf(-gate))) * up; }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -310,9 +338,17 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       const float sb = !kSplit && ok_b ? scales[kGateUp ? g.n_out + channel : channel_b] : 0.0f;
       // the tile's row scales while its MMAs still run: fetched chunk by chunk they cost two L2 round trips per 16 rows
       float* row_scale = mine->row_scale;
-      if constexpr (!kSplit)
-        for (int n = lane; n < t.n_eff; n += 32)
-          row_scale[n] = n < t.rows ? g.row_scale[t.row0 + n] : 0.0f;
+      bool far = false;
+      if constexpr (!kSplit) {
+        RowScales scales_here;
+        for (int n = lane; n < t.n_eff; n += 32) {
+          const float s = n < t.rows ? g.row_scale[t.row0 + n] : 0.0f;
+          row_scale[n] = s;
+          scales_here.add(s);
+        }
+        scales_here.join();
+        far = __any_sync(0xffffffffu, scales_here.far(sa) || scales_here.far(sb));
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(&c->tmem_full[acc], acc_phase, &c->abort, g.status))) break;
       __syncwarp();
       tc_fence_after();
@@ -336,35 +372,40 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
         // this team's part: one of the two boxes, or every other 16 rows
         constexpr bool kByBox = !kGateUp && kBoxes == 2 && kEpilogueWarps == 8;
         constexpr int kTeams = kEpilogueWarps / 4;
-        for (int n0 = kByBox ? 0 : team * 16; n0 < t.n_eff; n0 += kByBox ? 16 : 16 * kTeams) {
-          uint32_t a[16], b[16];
-          if (kByBox) {
-            tmem_ld16(taddr + (team ? token_tile : 0) + n0, a);
-          } else {
-            tmem_ld16(taddr + n0, a);
-            tmem_ld16(taddr + token_tile + n0, b);
-          }
-          float scale[16];
+        auto drain = [&](auto far_scales) {
+          constexpr bool kFar = decltype(far_scales)::value;
+          for (int n0 = kByBox ? 0 : team * 16; n0 < t.n_eff; n0 += kByBox ? 16 : 16 * kTeams) {
+            uint32_t a[16], b[16];
+            if (kByBox) {
+              tmem_ld16(taddr + (team ? token_tile : 0) + n0, a);
+            } else {
+              tmem_ld16(taddr + n0, a);
+              tmem_ld16(taddr + token_tile + n0, b);
+            }
+            float scale[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4*>(scale + 4 * j) = *reinterpret_cast<const float4*>(row_scale + n0 + 4 * j);
-          tmem_ld_wait();
-          float v[16];
-          const float s_mine = kByBox && team ? sb : sa;
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(scale + 4 * j) = *reinterpret_cast<const float4*>(row_scale + n0 + 4 * j);
+            tmem_ld_wait();
+            float v[16];
+            [[maybe_unused]] const float s_mine = kByBox && team ? sb : sa;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if constexpr (kGateUp) v[j] = swiglu(scaled(a[j], scale[j] * sa), scaled(b[j], scale[j] * sb));
-            else if constexpr (kBoxes == 1) v[j] = scaled(a[j] + b[j], scale[j] * sa);
-            else v[j] = scaled(a[j], scale[j] * s_mine);
-          }
-          const int channel0 = (kByBox && team ? channel_b : channel) - lane;
-          store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel0, g.n_out, mine->transpose, lane);
-          if constexpr (!kGateUp && kBoxes == 2 && !kByBox) {
+            for (int j = 0; j < 16; ++j) {
+              if constexpr (kGateUp) v[j] = swiglu(scaled<kFar>(a[j], scale[j], sa), scaled<kFar>(b[j], scale[j], sb));
+              else if constexpr (kBoxes == 1) v[j] = scaled<kFar>(a[j] + b[j], scale[j], sa);
+              else v[j] = scaled<kFar>(a[j], scale[j], s_mine);
+            }
+            const int channel0 = (kByBox && team ? channel_b : channel) - lane;
+            store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel0, g.n_out, mine->transpose, lane);
+            if constexpr (!kGateUp && kBoxes == 2 && !kByBox) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = scaled(b[j], scale[j] * sb);
-            store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel_b - lane, g.n_out, mine->transpose, lane);
+              for (int j = 0; j < 16; ++j) v[j] = scaled<kFar>(b[j], scale[j], sb);
+              store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel_b - lane, g.n_out, mine->transpose, lane);
+            }
           }
-        }
+        };
+        if (far) drain(std::true_type{});
+        else drain(std::false_type{});
       }
       tc_fence_before();
       __syncwarp();   // also: row_scale is read before the next tile's is written
@@ -419,8 +460,20 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
               sum[0] += v[b][i].x; sum[1] += v[b][i].y; sum[2] += v[b][i].z; sum[3] += v[b][i].w;
             }
           const float row_scale = split_rows[kRows == 2 ? min(n + b * stride, t.rows - 1) : n];
+          const float (&channel_scale)[4] = split_scale[kRows == 2 ? 0 : b];
+          float least = INFINITY, most = 0.0f;   // NaN passes: its products are NaN either way
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[b][j] = scaled(static_cast<uint32_t>(sum[j]), row_scale * split_scale[kRows == 2 ? 0 : b][j]);
+          for (int j = 0; j < 4; ++j) {
+            const float scale = row_scale * channel_scale[j];
+            y[b][j] = static_cast<float>(sum[j]) * scale;
+            least = fminf(least, fabsf(scale));
+            most = fmaxf(most, fabsf(scale));
+          }
+          if (!(least >= 0x1p-126f && most < INFINITY)) {
+            const float4 far = scaled_far4(make_int4(sum[0], sum[1], sum[2], sum[3]), row_scale,
+                                           make_float4(channel_scale[0], channel_scale[1], channel_scale[2], channel_scale[3]));
+            y[b][0] = far.x; y[b][1] = far.y; y[b][2] = far.z; y[b][3] = far.w;
+          }
         }
 #pragma unroll
         for (int b = 0; b < (kGateUp ? 1 : 2); ++b) {

@@ -40,6 +40,19 @@ __device__ __forceinline__ uint32_t top_bits(const float (&v)[8], uint32_t top) 
   return top;
 }
 
+// sum * row scale * channel scale. The product of the two scales comes first, one rounding (and in a tile one
+// multiplication) less per value. Where it leaves FP32's normal range, as with rows of 1e-35 and channels of 1e-6, the
+// result may still be in it; then the larger scale goes first. If the product is too small the larger is below 2^23
+// (nothing is below 2^-149) and |sum| below 2^31, so nothing overflows and only the last step may be subnormal; if it is
+// too large the result is an infinity, or 0 for a sum of 0. Selects and no branch: a second path costs short kernels more,
+// which fetch their instructions cold.
+__device__ __forceinline__ bool in_range(float scale) { return fabsf(scale) >= 0x1p-126f && fabsf(scale) < INFINITY; }
+__device__ __forceinline__ float scaled(int sum, float row, float channel) {
+  const float scale = row * channel;
+  const bool near = in_range(scale), channel_first = fabsf(channel) > row;
+  return static_cast<float>(sum) * (near ? scale : channel_first ? channel : row) * (near ? 1.0f : channel_first ? row : channel);
+}
+
 // The factors of a row whose largest magnitude has the bits `bits`.
 struct RowScale {
   float up;                          // a power of two that keeps the row clear of overflow and of subnormals

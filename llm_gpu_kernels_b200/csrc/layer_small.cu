@@ -105,12 +105,12 @@ layer_small_kernel(const LayerSmall a) {
     const size_t out = static_cast<size_t>(at) * a.n_out + n;
     if (kGateUp) {
       if (lane == 0) {
-        const float gate = static_cast<float>(s0) * (scale.scale * w_scale[n]);
-        const float up = static_cast<float>(s1) * (scale.scale * w_scale[n + second]);
+        const float gate = scaled(s0, scale.scale, w_scale[n]);
+        const float up = scaled(s1, scale.scale, w_scale[n + second]);
         a.y[out] = (gate / (1.0f + __expf(-gate))) * up;
       }
     } else if (lane < 2 && n + lane < a.n_out) {
-      a.y[out + lane] = static_cast<float>(lane ? s1 : s0) * (scale.scale * w_scale[n + lane]);
+      a.y[out + lane] = scaled(lane ? s1 : s0, scale.scale, w_scale[n + lane]);
     }
   }
 }

@@ -106,7 +106,7 @@ linear_small_kernel(const T* __restrict__ x, long long x_pitch, const int8_t* __
       for (int r = 0; r < kRows; ++r) {
         const int sum = __reduce_add_sync(0xffffffffu, acc[c][r]);
         if (lane == c * kRows + r && n0 + c < N && r < tokens)
-          store_out(y + static_cast<size_t>(r) * N + n0 + c, static_cast<float>(sum) * (row_scale[r] * w_scale[n0 + c]));
+          store_out(y + static_cast<size_t>(r) * N + n0 + c, scaled(sum, row_scale[r], w_scale[n0 + c]));
       }
   }
 }

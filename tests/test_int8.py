@@ -609,3 +609,58 @@ def test_rows_are_rounded_once(dev, t, e, k, h, i, tile):
     want, out = terms.sum(1), base.output.cpu().double()
     limit = HALF[torch.bfloat16] * want.abs() + (2.0 ** -21 + (k + 1) * 2.0 ** -24) * terms.abs().sum(1)
     assert not ((out - want).abs() > limit).any()
+
+
+# ---- scales whose product leaves the range of FP32 though the result does not
+def far_scales(t, k, n, dtype, g, exponents):
+    """x whose row maxima are near 2^exponents[0], a weight whose channel scales are near 2^exponents[1], in pairs such
+    that the results stay in the range of the type; and every third channel with a sum of zero."""
+    x = torch.randn(t, k, generator=g).clamp(-4, 4)
+    values = torch.randint(-127, 128, (n, k), dtype=torch.int8, generator=g)
+    values[::3] = 0
+    x, scales = x * 2.0 ** exponents[0], (1 + torch.rand(n, generator=g)) * 2.0 ** exponents[1]
+    return x.to(dtype), values, scales
+
+
+FAR = [   # BF16 rows (2^row) and channel scales (2^channel): products of the scales subnormal, zero or infinite in FP32
+    (-115, -25), (-118, -18), (-100, -42), (-60, -85), (-110, -45), (118, 30), (120, 126), (100, 60), (-90, -36)]
+
+
+@gpu
+@pytest.mark.parametrize("row,channel", FAR)
+@pytest.mark.parametrize("t,k,n", [(1, 600, 70), (2, 600, 70), (20, 600, 70), (20, 8192, 260), (130, 2048, 512), (300, 160, 129)])
+def test_scales_far_apart(dev, t, k, n, row, channel):
+    g = torch.Generator().manual_seed(t + k)
+    x, values, scales = far_scales(t, k, n, torch.bfloat16, g, (row, channel))
+    if row + channel > 100:
+        values[:] = 0            # any other sum leaves BF16
+        values[1, 0], values[1, 1] = 64, -64
+        x[:, 1] = x[:, 0]        # ... and two that cancel
+    if t > 2:
+        x[t // 2] = 0
+    want = Q.linear(x, values, scales)
+    p = prepare_int8_linear(x.to(dev), Int8Weight(values.to(dev), scales.to(dev)))
+    near(p.output, want, torch.bfloat16)
+    assert row + channel > 100 or (want != 0).any()
+
+
+@gpu
+@pytest.mark.parametrize("t,e,k", [(1, 4, 2), (40, 4, 2), (300, 3, 1)])
+@pytest.mark.parametrize("row,gate,up,down", [(-110, 117, -20, 30), (-110, 117, -14, -10), (110, -103, 30, 0)])
+def test_layer_scales_far_apart(dev, t, e, k, row, gate, up, down):
+    g = torch.Generator().manual_seed(t)
+    h, i = 256, 128
+    x = (torch.randn(t, h, generator=g).clamp(-4, 4) * 2.0 ** row).bfloat16()
+    values = torch.randint(-127, 128, (e, 2 * i, h), dtype=torch.int8, generator=g)
+    values[:, i + 5] = 0
+    if up > 0:
+        values[:, i:] = 0                        # any other sum leaves FP32
+    scales = (1 + torch.rand(e, 2 * i, generator=g))
+    scales[:, :i] *= 2.0 ** (gate - 17)          # sums of 256 products of two numbers up to 127 are some 2^17
+    scales[:, i:] *= 2.0 ** up
+    dvalues = torch.randint(-127, 128, (e, h, i), dtype=torch.int8, generator=g)
+    dscales = (1 + torch.rand(e, h, generator=g)) * 2.0 ** down
+    ids, rw = make_ids(t, e, k, "random", g).to(torch.int32), torch.rand(t, k, generator=g)
+    args = (x.to(dev), Int8Weight(values.to(dev), scales.to(dev)), Int8Weight(dvalues.to(dev), dscales.to(dev)),
+            ids.to(dev), rw.to(dev))
+    check_layer(prepare_int8_moe(*args), *args)
