@@ -30,6 +30,8 @@ struct LinearSmall {
   const int8_t* weight;
   const float* w_scale;
   void* y;
+  int8_t* q;           // the quantised rows and their scales, for whoever reads the workspace
+  float* q_scale;
   int dtype, tokens, k, n, sms;
 };
 bool linear_small_serves(int tokens, int k, int n);

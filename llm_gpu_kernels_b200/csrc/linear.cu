@@ -180,8 +180,8 @@ int b200moe_linear_forward(B200MoeLinear* p, void* cuda_stream) {
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (p->small) {
     const LinearSmall a{p->buf.x, p->shape.tokens > 1 ? p->buf.x_pitch : p->shape.k, static_cast<const int8_t*>(p->buf.weight),
-                        static_cast<const float*>(p->buf.weight_scale), p->buf.output, p->shape.dtype, p->shape.tokens,
-                        p->shape.k, p->shape.n, p->sms};
+                        static_cast<const float*>(p->buf.weight_scale), p->buf.output, static_cast<int8_t*>(p->buf.x_q),
+                        static_cast<float*>(p->buf.x_scale), p->shape.dtype, p->shape.tokens, p->shape.k, p->shape.n, p->sms};
     const cudaError_t e = launch_linear_small(a, s);
     if (e != cudaSuccess) {
       set_error("linear launch: %s", cudaGetErrorString(e));

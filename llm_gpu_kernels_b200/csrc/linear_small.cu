@@ -25,8 +25,8 @@ __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2hal
 template <typename T, int kRows, int kCh, bool kVec>
 __global__ void __launch_bounds__(kThreads)
 linear_small_kernel(const T* __restrict__ x, long long x_pitch, const int8_t* __restrict__ w,
-                    const float* __restrict__ w_scale, T* __restrict__ y, int tokens, int K, int N, int pitch,
-                    int smem_pitch) {
+                    const float* __restrict__ w_scale, T* __restrict__ y, int8_t* __restrict__ x_q,
+                    float* __restrict__ x_scale, int tokens, int K, int N, int pitch, int smem_pitch) {
   extern __shared__ __align__(16) unsigned char smem[];   // [kRows][smem_pitch] int8, zero past K
   __shared__ uint32_t part[kRows][kWarps];
   __shared__ float row_scale[kRows];
@@ -60,16 +60,20 @@ linear_small_kernel(const T* __restrict__ x, long long x_pitch, const int8_t* __
     if (lane == 0) part[r][warp] = bits[r];
   }
   __syncthreads();
+  const bool keep = blockIdx.x == 0;       // one block leaves the rows in memory too
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) bits[r] = max(bits[r], part[r][i]);
     const RowScale s = row_scale_of(bits[r]);
     if (threadIdx.x == r) row_scale[r] = s.scale;
+    if (keep && threadIdx.x == r && r < tokens) x_scale[r] = s.scale;
     for (int k = threadIdx.x * 8; k < smem_pitch; k += kThreads * 8) {
       float v[8] = {};
       if (r < tokens) load8<T, kVec>(x + r * x_pitch, k, K, v);
-      *reinterpret_cast<uint2*>(smem + r * smem_pitch + k) = quantize8<true>(v, s);
+      const uint2 q = quantize8<true>(v, s);
+      *reinterpret_cast<uint2*>(smem + r * smem_pitch + k) = q;
+      if (keep && k < pitch && r < tokens) *reinterpret_cast<uint2*>(x_q + static_cast<size_t>(r) * pitch + k) = q;
     }
   }
   __syncthreads();
@@ -122,9 +126,9 @@ cudaError_t launch(const LinearSmall& a, cudaStream_t s) {
   const int pitch = smem_pitch_of(a.k);
   const size_t smem = static_cast<size_t>(kRows) * pitch;
   return vec ? launch_pdl(linear_small_kernel<T, kRows, kCh, true>, grid, dim3(kThreads), smem, s, x, a.x_pitch, a.weight,
-                          a.w_scale, static_cast<T*>(a.y), a.tokens, a.k, a.n, int8_pitch(a.k), pitch)
+                          a.w_scale, static_cast<T*>(a.y), a.q, a.q_scale, a.tokens, a.k, a.n, int8_pitch(a.k), pitch)
              : launch_pdl(linear_small_kernel<T, kRows, kCh, false>, grid, dim3(kThreads), smem, s, x, a.x_pitch, a.weight,
-                          a.w_scale, static_cast<T*>(a.y), a.tokens, a.k, a.n, int8_pitch(a.k), pitch);
+                          a.w_scale, static_cast<T*>(a.y), a.q, a.q_scale, a.tokens, a.k, a.n, int8_pitch(a.k), pitch);
 }
 
 template <typename T>

@@ -664,3 +664,43 @@ def test_layer_scales_far_apart(dev, t, e, k, row, gate, up, down):
     args = (x.to(dev), Int8Weight(values.to(dev), scales.to(dev)), Int8Weight(dvalues.to(dev), dscales.to(dev)),
             ids.to(dev), rw.to(dev))
     check_layer(prepare_int8_moe(*args), *args)
+
+
+# ---- the quantised rows of one or two tokens, which the product without tensor cores makes itself
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,k", [(1, 72), (1, 1000), (1, 2048), (1, 9001), (1, 5), (2, 72), (2, 1000), (2, 2048), (2, 6000)])
+def test_quantised_rows_of_a_few_tokens(dev, dtype, t, k):
+    """Row by row the cases of test_quantised_rows_are_exact, in memory after a run and bit for bit what a batch gives."""
+    g = torch.Generator().manual_seed(t + k)
+    rows = torch.randn(10, k, generator=g)
+    rows[1] = torch.randint(-254, 255, (k,), generator=g) / 2.0
+    rows[1, 0] = 127.0
+    rows[2] = torch.randint(-127, 128, (k,), generator=g).float()
+    rows[2, k - 1] = -254.0
+    rows[3] = 0
+    rows[4] = 0
+    rows[4, k // 2] = -3e-5
+    rows[5] *= torch.finfo(dtype).max / 8
+    rows[6] *= torch.finfo(dtype).smallest_normal
+    rows[7] = rows[7].sign() * torch.finfo(dtype).tiny * 2.0 ** -6
+    rows[8] = -torch.finfo(dtype).max
+    rows[9] = torch.rand(k, generator=g) * 2.0 ** -7
+    rows = rows.to(dtype).to(dev)
+    w = quantize_int8(0.05 * torch.randn(70, k, generator=g)).to(dev)
+    x = rows[:t].clone()
+    p = prepare_int8_linear(x, w)
+    assert p.kernel_launches == 1
+    batch = prepare_int8_linear(rows, w)
+    for first in range(0, 10, t):
+        x.copy_(rows[first:first + t])
+        p.x_q.fill_(77)
+        p.x_scale.fill_(math.nan)
+        out = p.run()
+        q, _ = Q.quantize_rows(x.cpu())
+        assert torch.equal(p.x_q[:, :k].cpu().double(), q) and (p.x_q[:, k:] == 0).all()
+        assert torch.equal(p.x_scale.cpu(), x.cpu().float().abs().amax(-1) / 127)
+        assert torch.equal(out, batch.output[first:first + t])
+    x[t - 1, k // 2] = math.inf
+    p.run()
+    assert torch.isnan(p.x_scale[t - 1]) and (p.x_q[t - 1] == 0).all()
