@@ -498,7 +498,8 @@ __device__ __forceinline__ bool route_fast(const Config& cfg, float (&l)[P], con
       a = max(a, oa);
     }
     auto value_of = [&](uint32_t k) {
-      return exact ? K::value(k & ~255u) : base + static_cast<float>(static_cast<int>(k >> 8) - 2) * step;
+      // the last 8 bits of an exact logit are zeros: in the key of a negative one, which is inverted, they are ones
+      return exact ? K::value(k >> 31 ? k & ~255u : k | 255u) : base + static_cast<float>(static_cast<int>(k >> 8) - 2) * step;
     };
     auto far_below = [](uint32_t k) { return k < 512u; };   // q = 1; exact keys are larger
     const bool by_score = cfg.group_top2 && !biased;

@@ -590,3 +590,25 @@ def test_values_as_low_as_masks_in_groups(dev, score, group_score):
             l, b = l.to(dev), b.to(dev) if b is not None else None
             p = prepare_routing(l, 4, config=RouterConfig(**config), bias=b)
             agree(p.ids, p.routing_weights, l, 4, b, **config)
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("pairs", [1, 4])
+def test_groups_next_to_each_other(dev, score, dtype, pairs):
+    """Two groups of two experts whose sums of scores differ by a few millionths, logits of both signs."""
+    g = torch.Generator().manual_seed(31 + pairs)
+    two = (1.5 * torch.randn(200000, 2, generator=g)).to(dtype)
+    worth = (torch.exp(two.double()) if score == "softmax" else torch.sigmoid(two.double())).sum(1)
+    two = two[worth.argsort()[2000:198000]]
+    at = torch.randint(0, two.shape[0] - 1, (6000,), generator=g)
+    groups = torch.stack([two[at], two[at + 1]], 1)                                  # [rows, group, expert]
+    groups = torch.where(torch.rand(6000, 1, 1, generator=g) < 0.5, groups, groups.flip(1))
+    if pairs > 1:                                                                    # among groups that are far below
+        rest = torch.full((6000, 2 * pairs - 2, 2), -9.0, dtype=dtype)
+        groups = torch.cat([rest[:, :pairs], groups, rest[:, pairs:]], 1)
+    logits = groups.reshape(6000, -1).to(dev)
+    config = dict(score=score, groups=2 * pairs, kept_groups=1, group_score="top2")
+    p = prepare_routing(logits, 2, config=RouterConfig(**config))
+    agree(p.ids, p.routing_weights, logits, 2, **config)
