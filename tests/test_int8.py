@@ -704,3 +704,15 @@ def test_quantised_rows_of_a_few_tokens(dev, dtype, t, k):
     x[t - 1, k // 2] = math.inf
     p.run()
     assert torch.isnan(p.x_scale[t - 1]) and (p.x_q[t - 1] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("t,e,k,h,i,pattern", [(2100, 128, 8, 72, 40, "random"), (5000, 16, 4, 96, 33, "hot"), (17000, 3, 1, 40, 24, "random"),
+                                               (2049, 256, 8, 48, 16, "duplicate")])
+def test_layer_with_many_routes(dev, t, e, k, h, i, pattern):
+    """More routes than one launch of the dispatch ranks (16384): it takes three kernels and writes no rows."""
+    args = layer_inputs(t, e, k, h, i, pattern, dev, id_dtype=torch.int64 if t % 2 else torch.int32)
+    p = prepare_int8_moe(*args)
+    p.base.output.fill_(math.nan)
+    p.run()
+    check_layer(p, *args)
