@@ -85,7 +85,7 @@ struct EpilogueWarp {
   alignas(16) float row_scale[kMaxTile];                 // of the tile it works on
   alignas(16) unsigned char transpose[16 * kPitch];      // 16 rows of its 32 channels
 };
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 8;   // two teams of four, one warp per quarter of the TMEM lanes
 // Ctrl, and behind it what the epilogue needs: an EpilogueWarp each, or the row scales of a split tile.
 __host__ __device__ constexpr int ctrl_bytes(int out_bytes, bool split) {
   return kCtrlBytes + (split ? kMaxTile * 4
@@ -370,11 +370,10 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
       } else {
         Out* dst = static_cast<Out*>(g.out) + static_cast<size_t>(t.row0) * g.n_out;
         // this team's part: one of the two boxes, or every other 16 rows
-        constexpr bool kByBox = !kGateUp && kBoxes == 2 && kEpilogueWarps == 8;
-        constexpr int kTeams = kEpilogueWarps / 4;
+        constexpr bool kByBox = !kGateUp && kBoxes == 2;
         auto drain = [&](auto far_scales) {
           constexpr bool kFar = decltype(far_scales)::value;
-          for (int n0 = kByBox ? 0 : team * 16; n0 < t.n_eff; n0 += kByBox ? 16 : 16 * kTeams) {
+          for (int n0 = kByBox ? 0 : team * 16; n0 < t.n_eff; n0 += kByBox ? 16 : 32) {
             uint32_t a[16], b[16];
             if (kByBox) {
               tmem_ld16(taddr + (team ? token_tile : 0) + n0, a);
@@ -397,11 +396,6 @@ grouped_gemm_i8_kernel(const __grid_constant__ I8Gemm g) {
             }
             const int channel0 = (kByBox && team ? channel_b : channel) - lane;
             store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel0, g.n_out, mine->transpose, lane);
-            if constexpr (!kGateUp && kBoxes == 2 && !kByBox) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = scaled<kFar>(b[j], scale[j], sb);
-              store_rows(dst + static_cast<size_t>(n0) * g.n_out, v, t.rows - n0, channel_b - lane, g.n_out, mine->transpose, lane);
-            }
           }
         };
         if (far) drain(std::true_type{});

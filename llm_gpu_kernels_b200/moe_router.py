@@ -57,10 +57,10 @@ class RouterConfig:
     def kept(self):
         return self.groups if self.kept_groups is None else self.kept_groups
 
-    def native(self, bf16_weights=False):
+    def native(self):
         return _native.RouterConfig(score=SCORES[self.score], groups=self.groups, kept_groups=self.kept,
                                     group_score=GROUP_SCORES[self.group_score], renormalize=int(self.renormalize),
-                                    bf16_weights=int(bool(bf16_weights)), scale=self.scale)
+                                    scale=self.scale)
 
     def check(self, experts, topk):
         """Raises when ``topk`` experts cannot be chosen from ``experts`` in this way."""

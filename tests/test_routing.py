@@ -612,3 +612,16 @@ def test_groups_next_to_each_other(dev, score, dtype, pairs):
     config = dict(score=score, groups=2 * pairs, kept_groups=1, group_score="top2")
     p = prepare_routing(logits, 2, config=RouterConfig(**config))
     agree(p.ids, p.routing_weights, logits, 2, **config)
+
+
+@gpu
+@pytest.mark.parametrize("config", [{}, dict(score="sigmoid", groups=4, kept_groups=2, scale=2.5), dict(renormalize=False)])
+def test_library_rounds_weights_to_bf16(dev, config):
+    """A form that only the C entry has; inside a layer it is ``router_bf16_weights``."""
+    logits = make_logits(60, 64, torch.float32, 29, dev)
+    p = prepare_routing(logits, 6, config=RouterConfig(**config))
+    ids, weights = torch.zeros_like(p.ids), torch.zeros_like(p.routing_weights)
+    args = _native.RouteArgs.from_buffer_copy(p._args)
+    args.config.bf16_weights, args.ids, args.weights = 1, ids.data_ptr(), weights.data_ptr()
+    assert _native.load().b200moe_route(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(ids, p.ids) and torch.equal(weights, p.routing_weights.bfloat16().float())
