@@ -236,7 +236,7 @@ int b200moe_combine(B200MoePlan* plan, void* cuda_stream);
 /* Routing on logits that the caller has already (no counterpart in the reference, whose operator takes ids and
  * weights). ids = the K experts of the largest selection score in descending order, ties to the lower index; an
  * expert whose logit or bias is NaN or -inf is masked: never chosen while another is left, weight 0. The choice is
- * that of exact arithmetic on the logits; weights are FP32. Every row is written; nothing else is. No workspace:
+ * that of FP64 arithmetic on the logits; weights are FP32. Every row is written; nothing else is. No workspace:
  * calls may overlap on the GPU as long as their outputs differ. */
 typedef struct {
   int32_t tokens;          /* T >= 0 */

@@ -11,7 +11,8 @@
 //
 // gate/up: the two accumulators are the gate and the up rows of the same 128 channels; the epilogue scales both,
 // applies SwiGLU and stores FP32: the down product quantises these rows against their largest value, and rounding
-// them to BF16 first would move one in a hundred of the 8-bit values to its neighbour (0.8 % of the result). The rows of
+// them to BF16 first would move one in a hundred of the 8-bit values to its neighbour (normal gate and up: 1.6 % of them
+// at 768 channels, 1.0 % at 14336, by which the result moves 0.8 and 1.0 %). The rows of
 // a layer's down product stay FP32 as well, until the combine has summed them: the result is rounded once. As BF16 rows
 // they made a layer's error against 64 bits 0.0024 of the result instead of 0.0017, and saved a twentieth of its time at
 // most (1024 tokens of 128 experts 152.3 us, with FP32 rows 159.6; 2048 of 8 large ones 852 and 871).
@@ -33,9 +34,9 @@
 // and the output wait.
 //
 // Bound by: HBM while a group has few rows (the weights are streamed once: 604 MB for 128 experts of 2048 x 768, half of
-// BF16; with 64 rows each gate/up takes 80 us and reads 5.3 TB/s, the down product 42 us, 5.0 TB/s; its last round of
-// tiles fills a fifth of the SMs), by operand bytes through L2 and shared memory beyond (8192 x 4096 x 14336: 337 us in a
-// short burst, 2.86 POP/s, tensor pipe busy 72 % of its cycles; 404 us for seconds under the power limit).
+// BF16; with 64 rows each gate/up takes 80 us and reads 5.3 TB/s, the down product, which writes 67 MB of FP32 rows, 44 us;
+// the last round of tiles fills a fifth of the SMs), by operand bytes through L2 and shared memory beyond (8192 x 4096 x
+// 14336: 337 us in a short burst, 2.86 POP/s, tensor pipe busy 72 % of its cycles; 404 us for seconds under the power limit).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -144,6 +145,7 @@ struct RowScales {
     return channel != 0.0f && most != 0u && !(rows8::in_range(__uint_as_float(least) * channel) && rows8::in_range(__uint_as_float(most) * channel));
   }
 };
+// __expf: within 2^-22 + |gate| 2^-23, a thousandth of the step of 1 / 127 that the row is rounded to next.
 __device__ __forceinline__ float swiglu(float gate, float up) { return (gate / (1.0f + __expf(-gate))) * up; }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -534,8 +536,9 @@ int i8_stages(int out_bytes, int boxes, int token_tile, int split, int* smem_byt
   return stages;
 }
 
-// What decides between tile shapes, with figures fitted to 33 timings of 9 to 2048 rows (k 1999 to 4096, n 1536 to 5003;
-// all but four within 12 %). A stage takes the longest of its bytes at 50 bytes per cycle out of L2, its MMAs (half a
+// What decides between tile shapes: an estimate that has to rank them, not to tell the time. Its figures were fitted to 33
+// timings of 9 to 2048 rows (k 1999 to 4096, n 1536 to 5003) of an earlier form of the kernel, those of the epilogue with one
+// set of accumulators and of a split tile again when these changed, to the timings given here. A stage takes the longest of its bytes at 50 bytes per cycle out of L2, its MMAs (half a
 // cycle per row and K step of 32) and 210 cycles of hand-over; a tile that is not followed by another on its SM shows
 // its epilogue, 36 cycles per row and box; adding up a split tile takes 3200 cycles and 26 per row and box. Above 512
 // columns of accumulators there is only one set and every epilogue shows, at 30 cycles per row and box with eight warps:

@@ -6,7 +6,7 @@
 // of the tensor-core kernels to the bit.
 // Bound by the stream of weights, one pass per route (38 MB for 8 routes of 2048 x 768 experts: 5.8 us), and by the
 // launches: two kernels here against four (two quantisations, two products). Two blocks per SM: with three or four the
-// registers do not hold the weights in flight (1 token x 8 experts 20.8 and 24.6 us).
+// registers do not hold the weights in flight (1 token x 8 experts 20.8 and 24.6 us). __expf as in grouped_gemm_i8.cu.
 #include "int8.h"
 #include "int8_rows.cuh"
 #include "pdl.cuh"
@@ -131,8 +131,8 @@ cudaError_t launch(const LayerSmall& a, int sms, cudaStream_t s) {
 }  // namespace
 
 // One token of at most eight routes, two of at most two each: an expert's weights cross once per route here, once per
-// tile of rows there. A forward without / with tensor cores: 18.9 / 24.7 us for 1 token x 8 of 128 experts 2048 x 768,
-// 36.6 / 33.4 us for 2; 69 / 83, 109 / 123, 234 / 154 us for 1, 2, 3 tokens x 2 of 8 experts 4096 x 14336.
+// tile of rows there. A forward without / with tensor cores: 20.5 / 24.6 us for 1 token x 8 of 128 experts 2048 x 768,
+// 36.6 / 33.4 us for 2; 72 / 76, 107 / 105, 234 / 154 us for 1, 2, 3 tokens x 2 of 8 experts 4096 x 14336.
 bool layer_small_serves(int tokens, int topk, int hidden, int intermediate) {
   const int widest = hidden > intermediate ? hidden : intermediate;
   return ((tokens == 1 && topk <= 8) || (tokens == 2 && topk <= 2)) && widest <= 46 * 1024;

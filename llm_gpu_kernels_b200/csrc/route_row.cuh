@@ -11,21 +11,27 @@
 // An expert whose logit (or bias) is NaN or -inf is masked: no score, never chosen while another is left. Slots that
 // nobody can fill get the lowest indices not chosen yet, with weight 0, so the ids stay valid for the dispatch.
 //
-// Precision: the weights are FP32. The CHOICE is that of exact arithmetic: where c comes from exp() in FP32, two
-// values closer than the error bound of that computation could be in the wrong order. Where two neighbours of the order
+// Precision: the weights are FP32. The CHOICE is that of FP64, which is that of exact arithmetic unless two c, or two
+// groups, are closer than a few 2^-53 of their size: where c comes from exp() in FP32, two values closer than the error
+// bound of that computation could be in the wrong order. Where two neighbours of the order
 // (or the groups at the border) are that close, one row in a thousand for random logits, the experts found (the two
 // largest of each group) are put in order by their c in FP64, one expert per lane (exact_order, exact_groups). That is
 // enough if the next expert is not close as well; otherwise the whole row is routed in FP64 (route_exact). That pass
 // takes 9 us for a row, most of it instruction fetches, and a single late row shows in the call: with it alone 32768 rows
-// x 256 experts took 41.5 us instead of 35.5, 4099 x 160 masked 11.5 instead of 7.5.
+// x 256 experts took 41.5 us instead of 35.5, 4099 x 160 masked 11.5 instead of 7.5. Masks of -inf, NaN or a value below
+// -1e30 cost nothing. Finite ones in between stretch the range that the FP32 keys cover, -1e9 until no key tells one real
+// expert from another, and every row takes the long way: 32768 x 256 with a tenth of the logits at -1e9, softmax 123 us
+// instead of 25, with groups 373 instead of 40; with a tenth of the bias there, sigmoid 132 instead of 31, with groups 274
+// instead of 36.
 //
 // What bounds the common pass (route_fast) at many rows is the number of instructions per row, so it keeps the experts
 // of a lane as sorted 32-bit keys that hold the expert too: sorting eight is 19 compare-exchanges of two integer min /
 // max, each of the K rounds one maximum over the lanes and a shift of the winner's list. The K weights are computed at
 // the end by K lanes at once, from logits read again, so full-precision exp and division cost one instruction sequence
-// per row. 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups (5.4 us would be the HBM floor): 80 us with unsorted
+// per row. Only the sum that a softmax without renormalisation divides by is that of the choice, with __expf (within
+// 1.5e-6 of itself, see below): E more full exp per row would show, and the sum's own additions are as far off. 32768 rows x 256 experts FP32, sigmoid, bias, 8 groups (5.4 us would be the HBM floor): 80 us with unsorted
 // keys and per-expert weights (1930 warp instructions per row), 47 us with sorted keys that leave ties and experts to
-// ballots (910), 36 us like this (34.8 us if FP32 settled every row). Sixteen experts
+// ballots (910), 37 us like this (1018; 34.8 us if FP32 settled every row). Sixteen experts
 // per lane and two rows per warp need as many instructions per row (the warp-wide redux of 32 lanes becomes four
 // shuffles) and more registers: 73 us.
 #pragma once

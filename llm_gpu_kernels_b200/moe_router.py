@@ -12,7 +12,9 @@ the prepare functions runs without a ``router=``. Here the formula is a value:
     weights  the scores of those experts, divided by their sum if ``renormalize``, times ``scale``
 
 An expert whose logit (or bias) is NaN or -inf is masked: it has no score and is never chosen while another is left;
-slots that nobody can fill get the lowest unused indices with weight 0, so ids stay valid for the layer.
+slots that nobody can fill get the lowest unused indices with weight 0, so ids stay valid for the layer. Mask with -inf
+(or the type's lowest value, which keeps an expert as a last resort): a mask like -1e9 leaves FP32 no room between the
+other experts, and every row is routed in FP64, several times as long.
 
 ``prepare_routing`` routes logits a program already has; ``router=`` / ``router_bias=`` of ``prepare_moe`` and its
 siblings configure the router that computes them from ``router_weight``. ``run()`` of either only enqueues kernels on
