@@ -57,7 +57,8 @@ def forward(plan: int, x: torch.Tensor, weights: List[torch.Tensor], ids: torch.
     passed = [ids, routing_weights, output, *workspace]
     bound = _bound_tensors(prepared) if prepared is not None else passed
     if prepared is not None:
-        for given, real in ((x, prepared.x), (ids, prepared.ids), (routing_weights, prepared.routing_weights)):
+        for given, real in ((x, prepared.x), (ids, prepared.ids), (routing_weights, prepared.routing_weights),
+                            *zip(weights, prepared._op_args[2])):
             if given.data_ptr() != real.data_ptr():
                 real.copy_(given)
     if torch.cuda.current_device() == device.index:

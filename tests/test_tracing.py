@@ -113,3 +113,48 @@ def test_profiles_name_the_operators():
         with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as profile:
             run()
         assert f"b200moe::{name}" in [event.key for event in profile.key_averages()]
+
+
+@gpu
+@pytest.mark.parametrize("what", ["x", "ids", "residual", "router_bias", "router_weight", "logits", "bias", "linear"])
+def test_a_compiled_region_that_changes_an_input_runs_on_the_new_values(what):
+    """Under a functionalising compiler the change is a new tensor, which reaches the bound one only after the region."""
+    from llm_gpu_kernels_b200.int8_linear import prepare_int8_linear
+    from llm_gpu_kernels_b200.moe import prepare_moe
+    from llm_gpu_kernels_b200.moe_router import RouterConfig, prepare_routing
+    from tests.test_int8 import layer_inputs
+    dev = torch.device("cuda:0")
+    x, gate_up, down, ids, rw = layer_inputs(20, 8, 2, 128, 64, "random", dev)
+    plain = lambda w: w.dequantize().bfloat16()
+    g = torch.Generator().manual_seed(3)
+    if what in ("x", "ids", "residual"):
+        residual = torch.randn(20, 128, generator=g).bfloat16().to(dev)
+        prepared = prepare_moe(x, plain(gate_up), plain(down), ids, rw, residual=residual)
+        changed = {"x": x, "ids": ids, "residual": residual}[what]
+    elif what in ("router_bias", "router_weight"):
+        weight = torch.randn(8, 128, generator=g).bfloat16().to(dev)
+        bias = torch.zeros(8, device=dev)
+        prepared = prepare_moe(x, plain(gate_up), plain(down), ids, rw, router_weight=weight, router_bias=bias,
+                               router=RouterConfig(score="sigmoid"))
+        changed = bias if what == "router_bias" else weight
+    elif what in ("logits", "bias"):
+        logits, bias = torch.randn(20, 8, generator=g).to(dev), torch.zeros(8, device=dev)
+        prepared = prepare_routing(logits, 2, bias=bias)
+        changed = logits if what == "logits" else bias
+    else:
+        from llm_gpu_kernels_b200.int8_weights import Int8Weight
+        prepared = prepare_int8_linear(x, Int8Weight(gate_up.values[0], gate_up.scales[0]))
+        changed = x
+    first = lambda out: out[1] if isinstance(out, tuple) else out
+    other = (torch.flip(changed, [0]) + 1) % 8 if what == "ids" else torch.linspace(
+        -2, 2, changed.numel(), device=dev).view(changed.shape).to(changed.dtype)
+
+    def step(new):
+        changed.copy_(new)
+        return first(prepared.run()) * 1
+
+    before = first(prepared.run()).clone()
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(other)
+    assert torch.equal(changed, other)
+    want = first(prepared.run())
+    assert torch.equal(got, want) and not torch.equal(want, before)
